@@ -46,6 +46,11 @@ class MoePlanOut(C.Structure):
     _fields_ = [(n, C.c_uint64) for n in ("counts_va", "starts_va", "xmap_va", "ymap_va", "seg_a_va", "dir_a_va", "seg_b_va", "dir_b_va", "tiles_va", "header_va")]
 
 
+class MoeRouteConfig(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("experts", "topk", "score", "groups", "topk_groups", "group_rank", "norm_topk")] + [("weight_scale", C.c_float)]
+
+
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 assert C.sizeof(Fp8Info) == 160 and C.sizeof(Fp8GemmInfo) == 88
 
 VP = C.c_void_p
@@ -68,6 +73,15 @@ lib.omega_gpu_moe_layer_launches.argtypes = [VP]
 lib.omega_gpu_moe_layer_launches.restype = C.c_uint32
 lib.omega_gpu_moe_stack_launches.argtypes = [VP]
 lib.omega_gpu_moe_stack_launches.restype = C.c_uint32
+_U, _I, _V, _F = C.c_uint32, C.c_int, C.c_uint64, C.c_float   # device addresses and the stream of the 8-bit integer entries: plain integers
+for _n, _t in {"omega_gpu_moe_route_async": (C.POINTER(MoeRouteConfig), _U, _V, _I, _U, _V, _V, _V, VP), "omega_gpu_residual_norm_q8_async": (_U, _U, _F, _V, _V, _I, _V, _V, _V, _V, _V, _V, VP),
+               "omega_gpu_quant_q8_async": (_U, _U, _V, _I, _U, _V, _V, VP), "omega_gpu_swiglu_q8_async": (_U, _U, _V, _I, _V, _V, VP),
+               "omega_gpu_i8_gemm_async": (VP, _U, _V, _U, _V, _V, _V, VP), "omega_gpu_i8_gemm_grouped_async": (VP, _U, _U, _U, _V, _V, _V, _V, _V, _U, _V, _V, _V, VP),
+               "omega_gpu_moe_i8_layer_async": (VP, _U, _V, _V, _V, _V, VP), "omega_gpu_moe_i8_layer_q8_async": (VP, _U, _V, _V, _V, _V, _V, VP), "omega_gpu_i8_free": (VP,),
+               "omega_gpu_moe_i8_layer_free": (VP,), "omega_gpu_moe_i8_layer_launches": (VP,)}.items():
+    getattr(lib, _n).argtypes = _t
+lib.omega_gpu_i8_free.restype = lib.omega_gpu_moe_i8_layer_free.restype = None
+lib.omega_gpu_moe_i8_layer_launches.restype = C.c_uint32
 for _n in ("omega_moe_plan", "omega_moe_group", "omega_moe_ids32", "omega_moe_maps32", "omega_moe_segs32", "omega_moe_windows"):
     getattr(lib, _n).restype = C.c_uint32
 
@@ -374,3 +388,66 @@ def moe_router_f32(router, x, experts, eps=1e-6, norm_topk=True, out_scale=1.0, 
     rc = lib.omega_gpu_moe_router_f32(router, C.c_uint32(rows), _p(x), C.c_float(eps), C.c_int(1 if norm_topk else 0), C.c_float(out_scale), C.c_uint32(topk),
                                       _p(xn), _p(lg), _p(ids), _p(w))
     return rc, xn, lg, ids, w
+
+
+# ---------------------------------------------------------------- 8-bit integer path
+def moe_route(cfg, logits, bias=None):
+    """logits float32, or uint16 bf16 bits, [tokens][experts] -> (rc, ids, weights)"""
+    lg = np.ascontiguousarray(logits); bf16 = lg.dtype == np.uint16
+    lg = lg if bf16 else lg.astype(np.float32, copy=False)
+    b = None if bias is None else np.ascontiguousarray(bias, dtype=np.float32)
+    ids = np.empty((len(lg), cfg.topk), np.uint32); w = np.empty((len(lg), cfg.topk), np.float32)
+    rc = lib.omega_gpu_moe_route(C.byref(cfg), C.c_uint32(len(lg)), _p(lg), C.c_int(int(bf16)), _p(b), _p(ids), _p(w))
+    return rc, ids, w
+
+
+def residual_norm_q8_f32(x, m=None, norm_w=None, eps=1e-6):
+    """-> (rc, h, codes, scales)"""
+    x = np.ascontiguousarray(x, dtype=np.float32); T, H = x.shape
+    m = None if m is None else np.ascontiguousarray(m, dtype=np.float32); nw = None if norm_w is None else np.ascontiguousarray(norm_w, dtype=np.float32)
+    h = np.empty((T, H), np.float32); q = np.empty((T, H), np.int8); s = np.empty(T, np.float32)
+    rc = lib.omega_gpu_residual_norm_q8_f32(C.c_uint32(T), C.c_uint32(H), C.c_float(eps), _p(x), _p(m), _p(nw), _p(h), _p(q), _p(s))
+    return rc, h, q, s
+
+
+def swiglu_q8_f32(gu):
+    gu = np.ascontiguousarray(gu, dtype=np.float32); rows, two_i = gu.shape
+    q = np.empty((rows, two_i // 2), np.int8); s = np.empty(rows, np.float32)
+    return lib.omega_gpu_swiglu_q8_f32(C.c_uint32(rows), C.c_uint32(two_i // 2), _p(gu), _p(q), _p(s)), q, s
+
+
+def i8_upload(w, scale):
+    """w int8 [n][k], scale float32 [n] -> (rc, handle)"""
+    w = np.ascontiguousarray(w, dtype=np.int8); scale = np.ascontiguousarray(scale, dtype=np.float32)
+    h = VP()
+    rc = lib.omega_gpu_i8_upload(C.c_uint32(w.shape[0]), C.c_uint32(w.shape[1]), _p(w), _p(scale), C.byref(h))
+    return rc, (h if rc == 0 else None)
+
+
+def i8_upload_dev(n, k, w_va, scale_va):
+    h = VP()
+    rc = lib.omega_gpu_i8_upload_dev(C.c_uint32(n), C.c_uint32(k), C.c_uint64(w_va), C.c_uint64(scale_va), C.byref(h))
+    return rc, (h if rc == 0 else None)
+
+
+def i8_gemm(t, n, x, x_scale):
+    """x int8 [m][k] -> (rc, y as bf16 bits, y float32)"""
+    x = np.ascontiguousarray(x, dtype=np.int8); xs = np.ascontiguousarray(x_scale, dtype=np.float32)
+    y16 = _result((len(x), n), np.uint16); y32 = _result((len(x), n), np.float32)
+    return lib.omega_gpu_i8_gemm(t, C.c_uint32(len(x)), _p(x), _p(xs), _p(y16), _p(y32)), y16, y32
+
+
+def moe_i8_layer_create(gate_up, down, cfg, bias=None, max_tokens=256):
+    b = None if bias is None else np.ascontiguousarray(bias, dtype=np.float32)
+    h = VP()
+    rc = lib.omega_gpu_moe_i8_layer_create(gate_up, down, C.byref(cfg), _p(b), C.c_uint32(max_tokens), C.byref(h))
+    return rc, (h if rc == 0 else None)
+
+
+def moe_i8_layer_bf16(layer, logits_bf16, x_bf16, topk):
+    lg = np.ascontiguousarray(logits_bf16, dtype=np.uint16); x = np.ascontiguousarray(x_bf16, dtype=np.uint16)
+    T, H = x.shape
+    o16 = _result((T, H), np.uint16); o32 = _result((T, H), np.float32)
+    ids = np.empty((T, topk), np.uint32); w = np.empty((T, topk), np.float32)
+    rc = lib.omega_gpu_moe_i8_layer_bf16(layer, C.c_uint32(T), _p(lg), _p(x), _p(o16), _p(o32), _p(ids), _p(w))
+    return rc, o16, o32, ids, w

@@ -38,6 +38,9 @@ struct OmegaGpuW4Tensor {
     uint32_t gtiles, gn;   // omega_gpu_w4_gemm_grouped_async: most row tiles of a call, weight rows per expert; set by omega_gpu_w4_reserve_grouped
 };
 
+// 8-bit integer weight tensor (i8_gemm.cu): one matrix, or the matrices of several experts one after the other
+struct OmegaGpuI8Tensor { uint32_t n, k; int8_t *w; float *s; };
+
 namespace b200 {
 
 #define POISON_F32 (-999.0f)
@@ -65,6 +68,8 @@ State &st();
 void set_error(const char *fmt, ...);
 // true when the device is open (opens it on first use); false + last_error otherwise
 bool dev_open();
+// for the stream-ordered entries: OK when the device is open (opened on first use) and is the calling thread's current one
+int async_ready();
 // records a failing CUDA call; sticky errors latch the process
 bool cuda_ok(cudaError_t e, const char *what);
 // staging slot `i` with at least `bytes` (device memory); nullptr on failure
@@ -183,6 +188,19 @@ cudaError_t launch_w4_grouped(const OmegaGpuW4Tensor *t, uint32_t n, uint32_t ma
                               const uint16_t *x_bf16, uint16_t *y_bf16, float *y_f32, cudaStream_t s);
 bool ffn_shape_ok(uint32_t hidden, uint32_t inter);
 cudaError_t launch_ffn(const void *tm_gu, const void *tm_qx, const void *tm_dn, const void *tm_qa, uint32_t px, uint32_t pa, const FfnLaunch &m, cudaStream_t s, bool pdl);
+// ---- 8-bit integer path
+int score_route_ok(const OmegaGpuMoeRouteConfig *c);   // OK, or BAD_ARGS with the reason
+// stride: bytes between rows of logits, 0 = dense
+cudaError_t launch_score_route(const OmegaGpuMoeRouteConfig &c, uint32_t tokens, const void *logits, int bf16, size_t stride, const float *bias, uint32_t *ids, float *wts, cudaStream_t s);
+bool q8_length_ok(uint32_t n);                          // a row length that the two launchers below take
+cudaError_t launch_norm_q8(uint32_t tokens, uint32_t hidden, float eps, const void *x, int x_bf16, const void *m, int m_bf16, float *h, const float *nw, uint16_t *xn, int8_t *q, float *sc, cudaStream_t s);
+cudaError_t launch_row_q8(uint32_t rows, uint32_t n, size_t stride, const void *x, int x_bf16, int gate, int8_t *q, float *sc, cudaStream_t s);   // gate: silu(x[0 .. n)) * x[n .. 2n)
+// y = x W^T with both scales; n: weight rows of one expert (dense: all). tiles null: m dense rows; else a plan's tiles of at most tile_rows rows, at most m of them
+struct I8Launch {
+    uint32_t m, n; const int8_t *x; size_t x_stride; uint32_t x_rows; const float *xs; uint16_t *y16; float *y32;
+    const void *tiles; const uint32_t *header, *xmap, *ymap; uint32_t tile_rows;
+};
+cudaError_t launch_i8_gemm(const OmegaGpuI8Tensor *t, const I8Launch &a, cudaStream_t s);
 bool layer_forward(OmegaGpuMoeLayer *L, uint32_t tokens, const uint16_t *logits, const uint16_t *x, float *out32, uint16_t *out16, cudaStream_t s,
                    const uint32_t *ids_in = nullptr, const float *wts_in = nullptr);
 // expert side only (expert-parallel receive path): `rows` candidate rows, ids[row] = local expert or 0xFFFFFFFF,

@@ -50,6 +50,15 @@ bool dev_open() {
     return true;
 }
 
+int async_ready() {
+    State &g = st();
+    if (!g.opened) { Lock l; if (!dev_open()) return OMEGA_GPU_FP8_CHIP_FAIL; }
+    if (g.latched) return OMEGA_GPU_FP8_CHIP_FAIL;
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev != g.device) { (void)cudaGetLastError(); set_error("the current device is %d, the library's is %d", dev, g.device); return OMEGA_GPU_FP8_BAD_ARGS; }
+    return OMEGA_GPU_FP8_OK;
+}
+
 void *stage(int i, size_t bytes) {
     State &g = st();
     if (bytes == 0) bytes = 16;

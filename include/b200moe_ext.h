@@ -265,6 +265,88 @@ int omega_gpu_moe_router_rows_async(OmegaGpuMoeRouter *r, uint32_t rows, uint64_
 int omega_gpu_moe_router_f32(OmegaGpuMoeRouter *r, uint32_t rows, const float *x, float eps, int norm_topk, float out_scale, uint32_t topk,
                              float *xn, float *logits, uint32_t *ids, float *wts);
 
+/* ---- 8-bit integer path: rows and weights as signed 8-bit codes, one f32 scale for each row (token) and each weight row (channel). No counterpart in the
+ * reference. What a model quantised this way needs of an expert layer: routing by scores, residual + RMSNorm to 8-bit rows, the product, the SiLU gate to
+ * 8-bit rows, and the layer made of them. The _async entries open the library's device on first use; the calling thread's current device has to be that one
+ * (BAD_ARGS otherwise). */
+
+/* Routing by scores. Per token: score s_e = softmax over the experts or sigmoid of the logit (computed in 64 bits, rounded to f32); selection value
+ * c_e = s_e + bias_e (f32; bias f32 [experts] on the device, optional). With 1 < groups and topk_groups < groups, expert e belongs to group
+ * e / (experts / groups), a group's rank is the sum of its group_rank (1 or 2) largest c, and the topk_groups groups of largest rank are kept. The topk largest c
+ * of the kept groups are picked in descending order; equal values go to the lowest index, of groups and of experts. Weights: s_e of the picks, divided by
+ * (their sum + 1e-20) when norm_topk, times weight_scale. A NaN logit has score 0 and is picked behind every other expert of the kept groups (a NaN value
+ * counts as the lowest in its group's rank too); a logit of -infinity has score 0, and where every logit is -infinity or NaN all scores are 0. Logits of
+ * +infinity share the softmax equally. experts <= 1024, topk <= 32, groups <= 32 and divides experts, group_rank <= experts / groups,
+ * topk <= topk_groups * (experts / groups); a NaN bias counts as a NaN logit does, but for the score.
+ * The ids and weights are what omega_gpu_moe_plan_async and omega_gpu_moe_layer_routed_async take. */
+enum { OMEGA_GPU_MOE_SCORE_SOFTMAX = 0, OMEGA_GPU_MOE_SCORE_SIGMOID = 1 };
+typedef struct {
+    uint32_t experts, topk;
+    uint32_t score;          /* OMEGA_GPU_MOE_SCORE_* */
+    uint32_t groups;         /* 0 = 1 */
+    uint32_t topk_groups;    /* groups kept; 0 = all */
+    uint32_t group_rank;     /* 1 or 2; 0 = 1 */
+    uint32_t norm_topk;
+    float weight_scale;
+} OmegaGpuMoeRouteConfig;
+/* logits_va bf16 (logits_bf16 != 0) or f32 rows, logits_stride_bytes apart (0 = dense); ids_va u32 [tokens][topk], wts_va f32 [tokens][topk] */
+int omega_gpu_moe_route_async(const OmegaGpuMoeRouteConfig *cfg, uint32_t tokens, uint64_t logits_va, int logits_bf16, uint32_t logits_stride_bytes, uint64_t bias_va,
+                              uint64_t ids_va, uint64_t wts_va, void *stream);
+/* host buffers, dense */
+int omega_gpu_moe_route(const OmegaGpuMoeRouteConfig *cfg, uint32_t tokens, const void *logits, int logits_bf16, const float *bias, uint32_t *ids, float *wts);
+
+/* 8-bit rows: scale s = max(largest |y| of the row, 2^-100) / 127, codes round-to-nearest-even(y / s) in -127 .. 127. A row that holds a NaN or an infinity gets
+ * codes 0 and scale NaN, so that every product with it is NaN. Row lengths are multiples of 16, at most 16384; q_va int8 [rows][length], s_va f32 [rows]. Device
+ * addresses are 16-byte aligned (f32 scales 4). No output may overlap an input, except h_va = h_in_va. */
+/* h = (x16 ? bf16 -> f32(x16) : h_in) + (m ? m : 0); y = h / sqrt(mean(h^2) + eps) * norm_w, quantised. x16_va bf16 or h_in_va f32 [tokens][hidden] (one of them);
+ * m_va f32 or (m_bf16) bf16, optional; h_va f32, optional output; norm_w_va f32 [hidden], 0 = ones; xn_bf16_va optional output bf16(y), the rows that a router
+ * reads. Beside omega_gpu_residual_norm_w_async, which leaves bf16 rows. A row counts as non-finite when h * norm_w leaves the f32 range. */
+int omega_gpu_residual_norm_q8_async(uint32_t tokens, uint32_t hidden, float eps, uint64_t x16_va, uint64_t m_va, int m_bf16, uint64_t h_in_va, uint64_t h_va,
+                                     uint64_t norm_w_va, uint64_t xn_bf16_va, uint64_t q_va, uint64_t s_va, void *stream);
+/* rows as they are: x_va bf16 (x_bf16 != 0) or f32, x_stride_bytes apart (0 = dense; a multiple of 16) */
+int omega_gpu_quant_q8_async(uint32_t rows, uint32_t k, uint64_t x_va, int x_bf16, uint32_t x_stride_bytes, uint64_t q_va, uint64_t s_va, void *stream);
+/* silu(gate) * up, quantised: gu_va bf16 (gu_bf16 != 0) or f32 [rows][2 inter], gate columns first. Beside omega_gpu_swiglu_f32. */
+int omega_gpu_swiglu_q8_async(uint32_t rows, uint32_t inter, uint64_t gu_va, int gu_bf16, uint64_t q_va, uint64_t s_va, void *stream);
+/* host buffers, f32 inputs */
+int omega_gpu_residual_norm_q8_f32(uint32_t tokens, uint32_t hidden, float eps, const float *x, const float *m, const float *norm_w, float *h, int8_t *q, float *s);
+int omega_gpu_swiglu_q8_f32(uint32_t rows, uint32_t inter, const float *gu, int8_t *q, float *s);
+
+/* 8-bit integer weights: w int8 [n][k] (k a multiple of 16, at most 32768), scale f32 [n]; a NaN scale -> NAN_WEIGHT, an infinite one -> BAD_ARGS. Both are copied;
+ * the _dev form takes device addresses. Synchronous. */
+typedef struct OmegaGpuI8Tensor OmegaGpuI8Tensor;
+int omega_gpu_i8_upload(uint32_t n, uint32_t k, const int8_t *w, const float *scale, OmegaGpuI8Tensor **out);
+int omega_gpu_i8_upload_dev(uint32_t n, uint32_t k, uint64_t w_va, uint64_t scale_va, OmegaGpuI8Tensor **out);
+void omega_gpu_i8_free(OmegaGpuI8Tensor *t);
+/* y[i][j] = (sum over c of x[i][c] * w[j][c]) * (x_scale[i] * scale[j]): the sum is exact (32-bit integers), so a row's result does not depend on the other rows
+ * of its call. x_va int8 rows, x_stride_bytes apart (0 = dense; a multiple of 16, like x_va); y bf16 and / or f32 [m][n], dense. */
+int omega_gpu_i8_gemm_async(const OmegaGpuI8Tensor *t, uint32_t m, uint64_t x_va, uint32_t x_stride_bytes, uint64_t x_scale_va, uint64_t y_bf16_va, uint64_t y_f32_va,
+                            void *stream);
+/* host buffers, dense */
+int omega_gpu_i8_gemm(const OmegaGpuI8Tensor *t, uint32_t m, const int8_t *x, const float *x_scale, uint16_t *y_bf16, float *y_f32);
+/* Grouped by expert: the tensor was uploaded as experts x (n / experts) rows. The rows to multiply are described by a routing plan (omega_gpu_moe_plan_async) made
+ * with tile_rows from 1 to 256: tiles u32 x4 {expert, first sorted row, rows <= tile_rows, -}, header[2] = number of tiles, at most max_tiles. Row i of a tile is
+ * x[xmap[first + i]] with that row's scale (xmap_va 0: x[first + i]); x holds x_rows dense rows. Its result row (n / experts wide) is y[ymap[first + i]]
+ * (ymap_va 0: y[first + i]). One launch, nothing allocated. */
+int omega_gpu_i8_gemm_grouped_async(const OmegaGpuI8Tensor *t, uint32_t experts, uint32_t tile_rows, uint32_t max_tiles, uint64_t tiles_va, uint64_t header_va,
+                                    uint64_t xmap_va, uint64_t ymap_va, uint64_t x_va, uint32_t x_rows, uint64_t x_scale_va, uint64_t y_bf16_va, uint64_t y_f32_va, void *stream);
+
+/* ---- one MoE layer with 8-bit integer expert weights: routing by scores, plan, grouped gate|up rounded to bf16, SiLU gate to 8-bit rows, grouped down rounded to
+ * bf16, combine in slot order in f32. gate_up: experts x 2I rows of k = hidden (gate rows first, then up rows, per expert); down: experts x hidden rows of k = I; not
+ * owned by the layer, which they outlive; several layers may share them. bias f32 [experts] on the host (copied) or null. The layer owns its scratch: calls on one layer are
+ * ordered, by one stream or by the caller. */
+typedef struct OmegaGpuMoeI8Layer OmegaGpuMoeI8Layer;
+int omega_gpu_moe_i8_layer_create(const OmegaGpuI8Tensor *gate_up, const OmegaGpuI8Tensor *down, const OmegaGpuMoeRouteConfig *route, const float *bias, uint32_t max_tokens,
+                                  OmegaGpuMoeI8Layer **out);
+void omega_gpu_moe_i8_layer_free(OmegaGpuMoeI8Layer *l);
+/* logits bf16 [tokens][experts]; out f32 and / or bf16 [tokens][hidden]. x_va bf16 rows, quantised by the call; the _q8 form takes rows and scales as
+ * omega_gpu_residual_norm_q8_async leaves them */
+int omega_gpu_moe_i8_layer_async(OmegaGpuMoeI8Layer *l, uint32_t tokens, uint64_t logits_va, uint64_t x_va, uint64_t out_f32_va, uint64_t out_bf16_va, void *stream);
+int omega_gpu_moe_i8_layer_q8_async(OmegaGpuMoeI8Layer *l, uint32_t tokens, uint64_t logits_va, uint64_t q_va, uint64_t s_va, uint64_t out_f32_va, uint64_t out_bf16_va, void *stream);
+/* host buffers; ids / wts optional ([tokens][topk]) */
+int omega_gpu_moe_i8_layer_bf16(OmegaGpuMoeI8Layer *l, uint32_t tokens, const uint16_t *logits_bf16, const uint16_t *x_bf16, uint16_t *out_bf16, float *out_f32,
+                                uint32_t *ids, float *wts);
+uint32_t omega_gpu_moe_i8_layer_launches(const OmegaGpuMoeI8Layer *l);
+
 /* Measurement aid, no reference counterpart: the FP8 tensor throughput this GPU sustains when nothing has to be loaded (every SM
  * issues iters x 4 tcgen05 MMAs of M 128, N 256, K 32 on operands resident in shared memory). *tflops = best of `repeats` timed
  * launches (CUDA events), *ms_out (optional) that launch's duration. The denominator for "fraction of FP8 tensor peak". */
