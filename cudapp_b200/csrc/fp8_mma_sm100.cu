@@ -302,10 +302,10 @@ static EncodeTiledFn encode_fn() {
     return fn;
 }
 // 2-D map over a row-major u8 matrix [rows][cols], box [box_rows][128 bytes], 128-byte swizzle
-bool make_tmap_u8(void *out_map, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+bool make_tmap_u8(void *out_map, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows, uint64_t stride) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) { set_error("cuTensorMapEncodeTiled is not available from this driver"); return false; }
-    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols};
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {stride ? stride : cols};
     const cuuint32_t box[2] = {128, box_rows}, estr[2] = {1, 1};
     const CUresult r = fn((CUtensorMap *)out_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

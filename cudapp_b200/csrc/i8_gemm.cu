@@ -84,6 +84,8 @@ __global__ void __launch_bounds__(256) i8_rows_kernel(const I8Args a) {
 }
 
 cudaError_t launch_i8_gemm(const OmegaGpuI8Tensor *t, const I8Launch &l, cudaStream_t s) {
+    const uint32_t tall = l.tiles ? l.tile_rows : l.m;
+    if (tall > 16u) return launch_i8_mma(t, l, s);
     I8Args a = {};
     a.w = t->w; a.ws = t->s; a.x = l.x; a.xs = l.xs; a.y16 = l.y16; a.y32 = l.y32; a.x_stride = l.x_stride ? l.x_stride : t->k; a.m = l.m; a.n = l.n; a.k = t->k;
     a.tiles = (const uint4 *)l.tiles; a.header = l.header; a.xmap = l.xmap; a.ymap = l.ymap; a.blocks = (l.n + 15u) / 16u;
@@ -115,10 +117,12 @@ static int i8_make(uint32_t n, uint32_t k, const void *w, const void *scale, cud
     if (!t) return OMEGA_GPU_FP8_BAD_ARGS;
     t->n = n; t->k = k;
     cudaStream_t s = st().stream;
-    const bool ok = cuda_ok(cudaMalloc(&t->w, (size_t)n * k), "cudaMalloc(i8)") && cuda_ok(cudaMalloc(&t->s, (size_t)n * 4), "cudaMalloc(i8 scales)") &&
+    const bool ok = cuda_ok(cudaMalloc(&t->w, (size_t)n * k), "cudaMalloc(i8)") && cuda_ok(cudaMalloc(&t->s, (size_t)n * 4 + 16), "cudaMalloc(i8 scales)") &&
+                    cuda_ok(cudaMemsetAsync(t->s, 0, (size_t)n * 4 + 16, s), "memset") &&
                     cuda_ok(cudaMemcpyAsync(t->w, w, (size_t)n * k, kind, s), "copy i8") && cuda_ok(cudaMemcpyAsync(t->s, scale, (size_t)n * 4, kind, s), "copy i8 scales") &&
                     cuda_ok(cudaStreamSynchronize(s), "i8 upload");
     if (!ok) { if (t->w) cudaFree(t->w); if (t->s) cudaFree(t->s); free(t); return OMEGA_GPU_FP8_CHIP_FAIL; }
+    t->err = reinterpret_cast<uint32_t *>(t->s + n);
     *out = t;
     return OMEGA_GPU_FP8_OK;
 }

@@ -1,0 +1,415 @@
+// i8_mma_sm100.cu: the product of i8_gemm.cu on tcgen05 (kind::i8, 32-bit integer accumulators in TMEM), for more than a few rows.
+//
+// Weights are the M operand, activation rows the N operand: N follows a tile's row count in steps of 16 (32 for a pair of CTAs), so a ragged tile wastes no more than
+// that, and one kernel serves an expert's three rows and a prefill's 256. Accumulators need no promotion on the way through k: a unit of work (a tile of rows, a block of
+// 128 CG channels) runs its whole k into one accumulator and is drained once, while the next unit fills the other.
+//
+// What bounds it is shared memory: 128 columns of a 128 x 256 unit are written (48 KB) and read by four products (48 KB) at 128 bytes a clock, 750 clocks for 512 of
+// tensor work; measured 0.33 us. CG = 2: two CTAs share a unit of 256 channels; each holds its half of the channels and of the rows, the products read both halves, and a
+// row's bytes are written and read once for 256 channels: 0.25 us, the tensor cores' own rate (4096 x 4096 x 4096: 53 us with one CTA, 46 with two). Two blocks of
+// 128 channels per CTA instead save the writes but not the reads and leave no second accumulator: 52 us. GATHER: the rows of a tile are fetched through a row map by
+// four warps with 16-byte asynchronous copies (TMA's four-row gather takes 95 clocks a time: 308 us for the gate|up product of a 4096-token layer, whose rows in sorted order take 122).
+//
+// Warps: 0 weights (TMA), 1 MMA issuer (of a pair's first CTA), 2 TMEM, 3 rows (TMA), 4 - 19 epilogue,
+// GATHER 20 - 23 row copies. Every mbarrier wait is bounded; on expiry the kernel records a code in *err, lets its own copies land, frees its TMEM and returns, and
+// later launches on the tensor do nothing.
+#include <math.h>
+#include <stdlib.h>
+#include "internal.h"
+#include "mma_common.cuh"
+
+namespace b200 {
+
+constexpr uint32_t I8_EPI = 16, I8_STAGES = 12, I8_N_MAX = 256;   // epilogue warps, most stages, most rows of a tile
+constexpr uint32_t i8_threads(bool gather) { return 128 + 32 * I8_EPI + (gather ? 128 : 0); }
+constexpr uint32_t I8_OUT_ROW = 80, I8_OUT = 16 * I8_OUT_ROW;     // an epilogue warp's 16 result rows of 32 bf16 channels; 80 bytes apart: neither side meets a bank twice
+constexpr size_t I8_SMEM = 214 * 1024;                            // dynamic shared memory of every form: stages, result rows, alignment
+
+struct I8MmaArgs {
+    const float *ws, *xs; uint16_t *y16; float *y32;
+    const uint4 *tiles; const uint32_t *header, *xmap, *ymap;
+    const int8_t *x; size_t x_stride; uint32_t x_rows;             // GATHER
+    // n: channels of one matrix; n_cap: accumulator columns of a tile; box: rows of one load; packed: bf16 rows of a multiple of 8 channels; lag: of a copying warp's stages, how many stay in flight behind the newest, 0 or 1;
+    // early: the units and their weights are known before the kernels ahead in the stream have completed
+    uint32_t m, n, k, tile_rows, tiles_dense, cblocks, n_cap, stages, tmem_cols, box, packed, lag, early;
+    uint32_t *err;
+};
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{ .reg .pred q; elect.sync _|q, 0xffffffff; selp.u32 %0, 1, 0, q; }" : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t in_first_cta(uint32_t addr) { uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr)); return r; }
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// the bounded wait of mma_common.cuh, seeing what the other CTA of a pair released
+template <int CG> __device__ __forceinline__ bool i8_wait(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag, uint32_t *err, uint32_t code) {
+    if constexpr (CG == 1) return mbar_wait(bar, parity, abort_flag, err, code);
+    for (uint32_t i = 0; i < SPIN_LIMIT; i++) {
+        uint32_t ok;
+        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+        if ((i & 255u) == 255u && *abort_flag) return false;
+    }
+    *abort_flag = 1; atomicCAS(err, 0u, code);
+    return false;
+}
+template <int CG> __device__ __forceinline__ void i8_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
+    if constexpr (CG == 1) tma_load_2d(dst, map, bar, x, y);
+    else asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+template <int CG> __device__ __forceinline__ void i8_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (CG == 1) asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    else asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+template <int CG> __device__ __forceinline__ void i8_commit(uint32_t bar) {   // in both CTAs of a pair
+    if constexpr (CG == 1) tc_commit(bar);
+    else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+// 16 bytes to shared memory, zeros where `take` is 0
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t take) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take) : "memory"); }
+template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+// 16 TMEM lanes x 16 columns: registers 4 i + {0, 1} hold lane T / 4, columns 8 i + 2 (T % 4) + {0, 1}; 4 i + {2, 3} the lane 8 further on
+#define TMEM_LD16X256(taddr, r, o)                                                                                                       \
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"                                                 \
+                 : "=r"(r[o + 0]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7]) : "r"(taddr))
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) { uint32_t r; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo)); return r; }
+__device__ __forceinline__ void stmatrix_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void lds128(uint32_t addr, uint32_t (&v)[4]) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+}
+
+struct I8Unit { uint32_t expert, row0, cnt, c0; };
+// a place in a ring and the parity of its turn, without the divisions that a counter would need in every step (an issuer with them: 0.39 us per 128 columns, whatever the tile)
+struct I8Stage { uint32_t s = 0, phase = 0; __device__ __forceinline__ void next(uint32_t count) { if (++s == count) { s = 0; phase ^= 1u; } } };
+// Unit u is channel block u % cblocks of tile u / cblocks, and a worker takes every gridDim-th: the units in work at a time are those of neighbouring tiles, which share
+// their rows and, where an expert has several tiles, its weights. (In runs of consecutive units per worker, cut by cost, an expert's weights came from memory once per tile: a
+// 4096-token gate|up 159 us instead of 138.)
+template <int CG> __device__ __forceinline__ I8Unit i8_unit(const I8MmaArgs &a, uint32_t u) {
+    const uint32_t t = u / a.cblocks;
+    I8Unit r;
+    r.c0 = (u - t * a.cblocks) * (128u * CG);
+    if (a.tiles) { const uint4 v = a.tiles[t]; r.expert = v.x; r.row0 = v.y; r.cnt = v.z; }
+    else { r.expert = 0; r.row0 = t * a.tile_rows; r.cnt = min(a.tile_rows, a.m - r.row0); }
+    return r;
+}
+
+template <int CG, bool GATHER>
+__global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const I8MmaArgs a) {
+    extern __shared__ uint8_t dyn_smem[];
+    __shared__ __align__(8) uint64_t s_bar[2 * I8_STAGES + 5];
+    __shared__ uint32_t s_tmem, s_abort, s_total;
+    __shared__ __align__(16) float s_xs[2][I8_N_MAX];
+    __shared__ __align__(16) uint32_t s_row[2][I8_N_MAX];
+    __shared__ uint32_t s_src[GATHER ? 4 : 1][GATHER ? I8_N_MAX : 1];   // a copying warp's source rows of its unit
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, rank = CG == 2 ? cluster_rank() : 0u;
+    const uint32_t smem_base = (smem_u32(dyn_smem) + 1023u) & ~1023u;
+    const uint32_t bar0 = smem_u32(s_bar);
+    auto full_bar = [&](uint32_t s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](uint32_t s) { return bar0 + 8u * (I8_STAGES + s); };
+    auto accfull_bar = [&](uint32_t b) { return bar0 + 8u * (2 * I8_STAGES + b); };
+    auto accempty_bar = [&](uint32_t b) { return bar0 + 8u * (2 * I8_STAGES + 2 + b); };
+    const uint32_t all_bar = bar0 + 8u * (2 * I8_STAGES + 4);   // every epilogue warp; not bar.sync, which would wait for a warp that gave up
+    volatile uint32_t *abort_flag = &s_abort;
+    const uint32_t stage_bytes = A_TILE + a.n_cap / CG * 128u;
+
+    auto units = [&]() { return *reinterpret_cast<volatile uint32_t *>(a.err) ? 0u : (a.tiles ? a.header[2] : a.tiles_dense) * a.cblocks; };   // after a recorded failure: no work
+
+    if (threadIdx.x == 0) {
+        s_abort = 0;
+        if (a.early) s_total = units();
+        // a filled stage: one arrival for the weights and one for the rows (of a pair by the first CTA, for both)
+        for (uint32_t s = 0; s < I8_STAGES; s++) { mbar_init(full_bar(s), 2); mbar_init(empty_bar(s), 1); }
+        for (uint32_t b = 0; b < 2; b++) { mbar_init(accfull_bar(b), 1); mbar_init(accempty_bar(b), I8_EPI * CG); }
+        mbar_init(all_bar, I8_EPI);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        if constexpr (CG == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(a.tmem_cols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(a.tmem_cols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem, KB = (a.k + 127u) / 128u;
+    if (!a.early || warp != 0) griddep_chain();   // early weights are requested while the kernels ahead still run
+    const uint32_t total = a.early ? s_total : units();
+    const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
+    auto tile_rows = [](uint32_t cnt) { return (cnt + 16u * CG - 1u) / (16u * CG) * 16u; };   // rows of a tile that this CTA holds
+    auto filled_bar = [&](uint32_t s) { return CG == 2 ? in_first_cta(full_bar(s)) : full_bar(s); };
+
+    if (warp == 0) {
+        // ---------------------------------------------------------------- weights
+        I8Stage st; bool ok = true;
+        for (uint32_t u = first; u < total && ok; u += step) {
+            const I8Unit t = i8_unit<CG>(a, u);
+            const int wy = (int)(t.expert * a.n + t.c0 + rank * 128u);
+            for (uint32_t kb = 0; kb < KB; kb++, st.next(a.stages)) {
+                if (!(ok = i8_wait<CG>(empty_bar(st.s), st.phase ^ 1u, abort_flag, a.err, 1))) break;
+                if (elect_one()) {
+                    if (rank == 0) mbar_expect_tx(full_bar(st.s), CG * A_TILE);
+                    i8_load<CG>(smem_base + st.s * stage_bytes, &tm_w, filled_bar(st.s), (int)(kb * 128u), wy);
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- MMA issuer
+        // the whole warp walks through the loop, one lane issues: addresses and descriptors then stay in uniform registers
+        I8Stage st, acc; bool ok = rank == 0;   // acc: accumulator buffers
+        for (uint32_t u = first; u < total && ok; u += step, acc.next(2)) {
+            const I8Unit t = i8_unit<CG>(a, u);
+            const uint32_t cols = tile_rows(t.cnt) * CG, buf = acc.s;
+            // D s32, A = B = signed 8-bit, both K-major, M 128 CG, N cols
+            const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((cols >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
+            const uint32_t d = tmem + buf * a.n_cap;
+            if (!(ok = i8_wait<CG>(accempty_bar(buf), acc.phase ^ 1u, abort_flag, a.err, 2))) break;
+            tc_fence_after();
+            for (uint32_t kb = 0; kb < KB; kb++, st.next(a.stages)) {
+                if (!(ok = i8_wait<CG>(full_bar(st.s), st.phase, abort_flag, a.err, 3))) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t dw = umma_desc(smem_base + st.s * stage_bytes), dx = umma_desc(smem_base + st.s * stage_bytes + A_TILE);
+#pragma unroll
+                    for (uint32_t ks = 0; ks < 4; ks++) i8_mma<CG>(d, dw + 2u * ks, dx + 2u * ks, idesc, kb | ks);   // 32 columns each
+                    i8_commit<CG>(empty_bar(st.s));
+                }
+                __syncwarp();
+            }
+            if (ok && elect_one()) i8_commit<CG>(accfull_bar(buf));
+            __syncwarp();
+        }
+    } else if (warp == 3) {
+        // ---------------------------------------------------------------- activation rows
+        if constexpr (!GATHER) {
+            I8Stage st; bool ok = true;
+            for (uint32_t u = first; u < total && ok; u += step) {
+                const I8Unit t = i8_unit<CG>(a, u);
+                const uint32_t rows = tile_rows(t.cnt), boxes = (rows + a.box - 1u) / a.box;
+                const int y = (int)(t.row0 + rank * rows);
+                for (uint32_t kb = 0; kb < KB; kb++, st.next(a.stages)) {
+                    if (!(ok = i8_wait<CG>(empty_bar(st.s), st.phase ^ 1u, abort_flag, a.err, 6))) break;
+                    if (elect_one()) {
+                        if (rank == 0) mbar_expect_tx(full_bar(st.s), CG * boxes * a.box * 128u);
+                        for (uint32_t i = 0; i < boxes; i++) i8_load<CG>(smem_base + st.s * stage_bytes + A_TILE + i * a.box * 128u, &tm_x, filled_bar(st.s), (int)(kb * 128u), y + (int)(i * a.box));
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    } else if (warp >= 4 && warp < 4 + I8_EPI) {
+        // ---------------------------------------------------------------- epilogue: 32 channels and every fourth 16 rows per warp
+        const uint32_t et = threadIdx.x - 128u, quarter = warp & 3u, sub = (warp - 4u) >> 2, out_base = smem_base + a.stages * stage_bytes + (warp - 4u) * I8_OUT;
+        I8Unit next; float next_xs = 0.0f, next_w[4]; uint32_t next_row = 0;
+        auto fetch = [&](uint32_t u) {   // what a unit's drain needs from memory, a unit ahead
+            next = i8_unit<CG>(a, u);
+            if (et < next.cnt) {
+                const uint32_t r = next.row0 + et;
+                next_xs = a.xs[a.xmap ? a.xmap[r] : r];
+                next_row = a.ymap ? a.ymap[r] : r;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t ch = next.c0 + rank * 128u + quarter * 32u + (a.packed ? (lane >> 2) + 8u * i : lane);
+                next_w[i] = ch < a.n ? __ldg(a.ws + (size_t)next.expert * a.n + ch) : 0.0f;
+            }
+        };
+        if (first < total) fetch(first);
+        I8Stage acc; uint32_t n = 0; bool ok = true;
+        for (uint32_t u = first; u < total && ok; u += step, n++, acc.next(2)) {
+            const I8Unit t = next;
+            const uint32_t buf = acc.s, p = n & 1u;
+            if (et < t.cnt) { s_xs[p][et] = next_xs; s_row[p][et] = next_row; }
+            float w[4];   // packed: channels lane / 4 + 0, 8, 16, 24 of the warp's 32; else [0]: channel lane
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = next_w[i];
+            if (u + step < total) fetch(u + step);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(all_bar);
+            if (!(ok = mbar_wait(all_bar, n & 1u, abort_flag, a.err, 5))) break;
+            if (!(ok = i8_wait<CG>(accfull_bar(buf), acc.phase, abort_flag, a.err, 4))) break;
+            tc_fence_after();
+            const uint32_t taddr = tmem + ((quarter * 32u) << 16) + buf * a.n_cap, ch0 = t.c0 + rank * 128u + quarter * 32u;
+            if (a.packed) {
+                // a thread holds two neighbouring rows of a channel per register pair; the transposing store makes them 16-byte runs of a row's channels
+                uint32_t v[16];
+                const uint32_t part = lane & 3u, piece_ch = ch0 + part * 8u;
+                if (sub * 16u < t.cnt) { TMEM_LD16X256(taddr + sub * 16u, v, 0); TMEM_LD16X256(taddr + (16u << 16) + sub * 16u, v, 8); }
+                for (uint32_t c = sub * 16u; c < t.cnt; c += 64u) {
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    uint32_t o[8];
+                    const float2 x0 = *reinterpret_cast<const float2 *>(&s_xs[p][c + 2u * part]), x1 = *reinterpret_cast<const float2 *>(&s_xs[p][c + 8u + 2u * part]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {   // 8 channels x 8 rows each: i & 1 the second eight channels, i >> 1 the second eight rows of the 16 x 16 block
+                        const float2 x = i >> 1 ? x1 : x0;
+                        o[i] = pack_bf16((float)(int)v[2 * i] * (x.x * w[i & 1]), (float)(int)v[2 * i + 1] * (x.y * w[i & 1]));
+                        o[4 + i] = pack_bf16((float)(int)v[8 + 2 * i] * (x.x * w[2 + (i & 1)]), (float)(int)v[8 + 2 * i + 1] * (x.y * w[2 + (i & 1)]));
+                    }
+                    if (c + 64u < t.cnt) { TMEM_LD16X256(taddr + c + 64u, v, 0); TMEM_LD16X256(taddr + (16u << 16) + c + 64u, v, 8); }
+                    const uint32_t at = out_base + ((lane >> 4) * 8u + (lane & 7u)) * I8_OUT_ROW + ((lane >> 3) & 1u) * 16u;
+                    stmatrix_trans(at, o[0], o[1], o[2], o[3]);
+                    stmatrix_trans(at + 32u, o[4], o[5], o[6], o[7]);
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const uint32_t j = (lane >> 2) + 8u * i;
+                        uint32_t q[4]; lds128(out_base + j * I8_OUT_ROW + part * 16u, q);
+                        if (c + j < t.cnt && piece_ch < a.n) *reinterpret_cast<uint4 *>(a.y16 + (size_t)s_row[p][c + j] * a.n + piece_ch) = make_uint4(q[0], q[1], q[2], q[3]);
+                    }
+                    __syncwarp();
+                }
+            } else {
+                for (uint32_t c = sub * 16u; c < t.cnt; c += 64u) {
+                    uint32_t v[16];
+                    TMEM_LD16(taddr + c, v, 0);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (ch0 + lane < a.n) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; i++) {
+                            if (c + i >= t.cnt) break;
+                            const float y = (float)(int)v[i] * (s_xs[p][c + i] * w[0]);
+                            const size_t at = (size_t)s_row[p][c + i] * a.n + ch0 + lane;
+                            if (a.y16) a.y16[at] = (uint16_t)bf16_rne_bits(y);
+                            if (a.y32) a.y32[at] = y;
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) { if constexpr (CG == 2) mbar_arrive_cluster(in_first_cta(accempty_bar(buf))); else mbar_arrive(accempty_bar(buf)); }
+        }
+    } else if (GATHER && warp >= 4 + I8_EPI) {
+        // ---------------------------------------------------------------- row copies: each of `team` warps fills every team-th stage
+        // No more warps than stages: a warp that waits for a place in the ring has then had one since the place's last turn began, and the barrier's parity tells the turns apart.
+        constexpr uint32_t team = 4;
+        static_assert((I8_SMEM - 1024 - I8_EPI * I8_OUT) / (A_TILE + I8_N_MAX * 128) >= team, "a ring of as many stages as copying warps");
+        // A stage is passed on once its copies have landed and are fenced for the tensor cores' reads; a.lag = 1: when the warp's next stage has been requested,
+        // which takes more than 2 * team stages in the ring (every wait for a free stage is then for one that has been passed on).
+        if constexpr (GATHER) {
+            const uint32_t me = warp - (4 + I8_EPI), c = lane & 7u, r0 = lane >> 3;
+            uint32_t *src = s_src[me];
+            I8Stage st, done; bool ok = true, behind = false;
+            uint32_t ahead[I8_N_MAX / 32], turn = 0;   // turn: stages until this warp's next
+            for (uint32_t i = 0; i < me; i++) st.next(a.stages);
+            done = st; turn = me;
+            auto fetch = [&](uint32_t u) {
+                const I8Unit t = i8_unit<CG>(a, u);
+#pragma unroll
+                for (uint32_t i = 0; i < I8_N_MAX / 32; i++) if (32u * i < t.cnt) ahead[i] = a.xmap[t.row0 + min(lane + 32u * i, t.cnt - 1u)];   // rows past the tile: any row, its columns are not read
+                return tile_rows(t.cnt);
+            };
+            auto pass_on = [&]() {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full_bar(done.s));
+                for (uint32_t i = 0; i < team; i++) done.next(a.stages);
+            };
+            uint32_t rows = first < total ? fetch(first) : 0u;
+            for (uint32_t u = first; u < total && ok; u += step) {
+                const uint32_t have = rows;
+                __syncwarp();
+#pragma unroll
+                for (uint32_t i = 0; i < I8_N_MAX / 32; i++) if (32u * i < have) src[lane + 32u * i] = min(ahead[i], a.x_rows - 1u);
+                __syncwarp();
+                if (u + step < total) rows = fetch(u + step);   // a unit ahead: the map's values are there when they are needed
+                for (uint32_t kb = turn; kb < KB; kb += team) {
+                    if (!(ok = __all_sync(0xffffffffu, i8_wait<CG>(empty_bar(st.s), st.phase ^ 1u, abort_flag, a.err, 7)))) break;
+                    const uint32_t dst = smem_base + st.s * stage_bytes + A_TILE + r0 * 128u, at = kb * 128u + c * 16u, take = at < a.k ? 16u : 0u;
+                    const int8_t *from = a.x + (take ? at : 0u);
+                    // the 128-byte swizzle: 16-byte column c of row r lies at column c ^ (r % 8)
+#pragma unroll 8
+                    for (uint32_t r = r0; r < have; r += 4u) copy16(dst + (r - r0) * 128u + ((c ^ (r & 7u)) << 4), from + (size_t)src[r] * a.x_stride, take);
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    if (a.lag == 0u) { copies_wait<0>(); pass_on(); }
+                    else if (behind) { copies_wait<1>(); pass_on(); }
+                    else behind = true;
+                    for (uint32_t i = 0; i < team; i++) st.next(a.stages);
+                }
+                turn = (turn + team - KB % team) % team;   // this warp's first stage of the next unit
+            }
+            copies_wait<0>();
+            if (ok && behind) pass_on();
+        }
+    }
+    // ---------------------------------------------------------------- teardown
+    if (*abort_flag) { for (int i = 0; i < 64; i++) __nanosleep(1000); }   // let copies already issued land before the CTA goes away
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync();   // the pair's products read this CTA's memory and arrive on its barriers
+    if (warp == 2) {
+        if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+    }
+}
+
+template <int CG, bool GATHER>
+static cudaError_t i8_mma_start(const CUtensorMap &w, const CUtensorMap &x, const I8MmaArgs &a, uint32_t grid, cudaStream_t s) {
+    auto kernel = i8_mma_kernel<CG, GATHER>;
+    // set on every call: it belongs to the device's context and costs well under a launch
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)I8_SMEM);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {}; cudaLaunchAttribute at[2];
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(i8_threads(GATHER)); cfg.dynamicSmemBytes = I8_SMEM; cfg.stream = s; cfg.attrs = at; cfg.numAttrs = CG;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension; at[1].val.clusterDim.x = 2; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, w, x, a);
+}
+
+// Form and tile of a dense product: the least of rounds * (the slower of a unit's mainloop and drain) + one drain, in us, over tile counts that divide the rows evenly.
+// Per 128 columns, measured with n rows in a tile: one CTA 0.22 + 0.00042 n and at least 0.27, a pair 0.15 + 0.0004 n and at least 0.19; draining a 128 x n accumulator
+// 0.5 + 0.013 n while all SMs store.
+static void i8_dense_form(uint32_t m, uint32_t n, uint32_t k, uint32_t sms, uint32_t *cg, uint32_t *rows) {
+    const float kb = (float)((k + 127u) / 128u);
+    float best = 3.4e38f;
+    for (uint32_t g = 1; g <= 2; g++) {
+        const uint32_t blocks = (n + 128u * g - 1u) / (128u * g), least = (m + I8_N_MAX - 1u) / I8_N_MAX, workers = sms / g;
+        for (uint32_t t = least; t < least + 24u && t <= m; t++) {
+            const uint32_t r = ((m + t - 1u) / t + 16u * g - 1u) / (16u * g) * (16u * g);
+            const float each = g == 1u ? fmaxf(0.27f, 0.22f + 0.00042f * r) : fmaxf(0.19f, 0.15f + 0.0004f * r), drain = 0.5f + 0.013f * r;
+            const float rounds = ceilf((float)((m + r - 1u) / r) * blocks / workers), cost = rounds * fmaxf(kb * each, drain) + drain;
+            if (cost < best) { best = cost; *cg = g; *rows = r; }
+        }
+    }
+}
+
+cudaError_t launch_i8_mma(const OmegaGpuI8Tensor *t, const I8Launch &l, cudaStream_t s) {
+    const uint32_t sms = st().sm_count ? st().sm_count : 148;
+    I8MmaArgs a = {};
+    a.ws = t->s; a.xs = l.xs; a.y16 = l.y16; a.y32 = l.y32; a.tiles = (const uint4 *)l.tiles; a.header = l.header; a.xmap = l.xmap; a.ymap = l.ymap;
+    a.m = l.m; a.n = l.n; a.k = t->k; a.err = t->err; a.x = l.x; a.x_stride = l.x_stride ? l.x_stride : t->k; a.x_rows = l.x_rows; a.early = !l.tiles || l.early;
+    uint32_t cg = 1;
+    if (l.tiles) { a.tile_rows = l.tile_rows; a.n_cap = (l.tile_rows + 15u) / 16u * 16u; }   // an expert's tiles: one CTA (gate|up of 4096 tokens: 122 us, 117 - 123 in pairs; down: 80 and 92)
+    else {
+        i8_dense_form(l.m, l.n, t->k, sms, &cg, &a.tile_rows);
+        const char *env = getenv("I8_FORM"); if (env) cg = atoi(env) + 1; env = getenv("I8_N"); if (env) a.tile_rows = atoi(env);   // development
+        a.n_cap = a.tile_rows; a.tiles_dense = (l.m + a.tile_rows - 1u) / a.tile_rows;
+    }
+    a.cblocks = (l.n + 128u * cg - 1u) / (128u * cg);
+    const uint32_t per_cta = a.n_cap / cg;
+    a.box = !l.tiles ? per_cta : per_cta % 64u == 0 ? 64u : per_cta % 32u == 0 ? 32u : 16u;
+    a.packed = l.y16 && !l.y32 && l.n % 8u == 0;
+    a.stages = (uint32_t)((I8_SMEM - 1024 - I8_EPI * I8_OUT) / (A_TILE + per_cta * 128u)); if (a.stages > I8_STAGES) a.stages = I8_STAGES;
+    a.lag = a.stages > 7u;
+    a.tmem_cols = 32; while (a.tmem_cols < 2u * a.n_cap) a.tmem_cols *= 2;
+    CUtensorMap w, x;
+    if (!make_tmap_u8(&w, t->w, t->n, t->k, 128) || !make_tmap_u8(&x, l.x, l.x_rows, t->k, a.box, l.x_stride)) return cudaErrorInvalidValue;
+    const uint64_t units = (uint64_t)(l.tiles ? l.m : a.tiles_dense) * a.cblocks;
+    if (units > 0x7fffffffull) return cudaErrorInvalidValue;
+    uint32_t grid = (uint32_t)(units * cg < sms ? units * cg : sms); grid -= grid % cg;
+    if (cg == 2u) return i8_mma_start<2, false>(w, x, a, grid, s);
+    return l.xmap ? i8_mma_start<1, true>(w, x, a, grid, s) : i8_mma_start<1, false>(w, x, a, grid, s);
+}
+
+}  // namespace b200

@@ -39,7 +39,7 @@ struct OmegaGpuW4Tensor {
 };
 
 // 8-bit integer weight tensor (i8_gemm.cu): one matrix, or the matrices of several experts one after the other
-struct OmegaGpuI8Tensor { uint32_t n, k; int8_t *w; float *s; };
+struct OmegaGpuI8Tensor { uint32_t n, k; int8_t *w; float *s; uint32_t *err; };   // err: device word, the code of a bounded wait that ran out
 
 namespace b200 {
 
@@ -167,7 +167,7 @@ struct MmaLaunch {
     const unsigned long long *gate; const uint64_t *out_peers, *ret_counters; uint32_t rows_per_rank, ret_index; const unsigned long long *gate_base; unsigned long long *bump;
     uint32_t wait_limit;               // iterations of the bounded wait on `gate` (0 = the default)
 };
-bool make_tmap_u8(void *out_map, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows);
+bool make_tmap_u8(void *out_map, const void *base, uint64_t rows, uint64_t cols, uint32_t box_rows, uint64_t stride = 0);   // stride: bytes between rows, 0 = cols
 uint32_t mma_tile_rows(uint32_t pieces);
 bool mma_shape_ok(uint32_t n, uint32_t k, uint32_t mode);
 cudaError_t launch_mma_grouped(const void *tm_w, const void *tm_q, uint32_t pieces, const MmaLaunch &m, cudaStream_t s, bool pdl = false);
@@ -199,8 +199,10 @@ cudaError_t launch_row_q8(uint32_t rows, uint32_t n, size_t stride, const void *
 struct I8Launch {
     uint32_t m, n; const int8_t *x; size_t x_stride; uint32_t x_rows; const float *xs; uint16_t *y16; float *y32;
     const void *tiles; const uint32_t *header, *xmap, *ymap; uint32_t tile_rows;
+    int early;   // the plan was complete before the launch ahead of this one began
 };
 cudaError_t launch_i8_gemm(const OmegaGpuI8Tensor *t, const I8Launch &a, cudaStream_t s);
+cudaError_t launch_i8_mma(const OmegaGpuI8Tensor *t, const I8Launch &a, cudaStream_t s);   // i8_mma_sm100.cu
 bool layer_forward(OmegaGpuMoeLayer *L, uint32_t tokens, const uint16_t *logits, const uint16_t *x, float *out32, uint16_t *out16, cudaStream_t s,
                    const uint32_t *ids_in = nullptr, const float *wts_in = nullptr);
 // expert side only (expert-parallel receive path): `rows` candidate rows, ids[row] = local expert or 0xFFFFFFFF,

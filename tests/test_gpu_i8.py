@@ -354,7 +354,7 @@ def test_layer(T, E, H, I, K, groups, kept, rank):
     assert np.array_equal(ids, wids) and np.all(np.abs(w - ww) <= (K + 5) * EPS24 * ww)
     assert np.linalg.norm(o32 - want) <= LAYER_REL * np.linalg.norm(want)
     assert np.all(np.abs(api.bf16_to_f32(o16) - o32) <= BF16_HALF * np.abs(o32))
-    assert api.lib.omega_gpu_moe_i8_layer_launches(L.h) == 7
+    assert api.lib.omega_gpu_moe_i8_layer_launches(L.h) == 7 + (T * K // E >= 32)             # one more copies the rows into sorted order
     # fewer tokens than the layer has room for: the same rows
     if T > 3:
         rc, _, p32, _, _ = api.moe_i8_layer_bf16(L.h, lg[1:4], x[1:4], K); ok(rc)
