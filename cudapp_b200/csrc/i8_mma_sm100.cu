@@ -9,6 +9,8 @@
 // row's bytes are written and read once for 256 channels: 0.25 us, the tensor cores' own rate (4096 x 4096 x 4096: 53 us with one CTA, 46 with two). Two blocks of
 // 128 channels per CTA instead save the writes but not the reads and leave no second accumulator: 52 us. GATHER: the rows of a tile are fetched through a row map by
 // four warps with 16-byte asynchronous copies (TMA's four-row gather takes 95 clocks a time: 308 us for the gate|up product of a 4096-token layer, whose rows in sorted order take 122).
+// SPLIT: where units are fewer than SMs, a cluster of 2, 4 or 8 CTAs shares one: each takes its part of k, leaves its sums in its shared memory, and adds up its share of the
+// rows over the cluster. Integer sums: the result is the same, whatever the split.
 //
 // Warps: 0 weights (TMA), 1 MMA issuer (of a pair's first CTA), 2 TMEM, 3 rows (TMA), 4 - 19 epilogue,
 // GATHER 20 - 23 row copies. Every mbarrier wait is bounded; on expiry the kernel records a code in *err, lets its own copies land, frees its TMEM and returns, and
@@ -30,8 +32,9 @@ struct I8MmaArgs {
     const uint4 *tiles; const uint32_t *header, *xmap, *ymap;
     const int8_t *x; size_t x_stride; uint32_t x_rows;             // GATHER
     // n: channels of one matrix; n_cap: accumulator columns of a tile; box: rows of one load; packed: bf16 rows of a multiple of 8 channels; lag: of a copying warp's stages, how many stay in flight behind the newest, 0 or 1;
+    // split: CTAs of a unit
     // early: the units and their weights are known before the kernels ahead in the stream have completed
-    uint32_t m, n, k, tile_rows, tiles_dense, cblocks, n_cap, stages, tmem_cols, box, packed, lag, early;
+    uint32_t m, n, k, tile_rows, tiles_dense, cblocks, n_cap, stages, tmem_cols, box, packed, lag, early, split;
     uint32_t *err;
 };
 
@@ -83,6 +86,24 @@ __device__ __forceinline__ void lds128(uint32_t addr, uint32_t (&v)[4]) {
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
 }
 
+// four sums and four of 64 channels further on at the same place of S CTAs' shared memory; all loads are on their way before the first is used
+template <int S> __device__ __forceinline__ void i8_sum_parts(uint32_t addr, int (&sum)[8]) {
+    int v[S][8];
+#pragma unroll
+    for (uint32_t r = 0; r < S; r++) {
+        uint32_t from;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(addr), "r"(r));
+        asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[r][0]), "=r"(v[r][1]), "=r"(v[r][2]), "=r"(v[r][3]) : "r"(from) : "memory");
+        asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[r][4]), "=r"(v[r][5]), "=r"(v[r][6]), "=r"(v[r][7]) : "r"(from + 256u) : "memory");
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        sum[i] = 0;
+#pragma unroll
+        for (int r = 0; r < S; r++) sum[i] += v[r][i];
+    }
+}
+
 struct I8Unit { uint32_t expert, row0, cnt, c0; };
 // a place in a ring and the parity of its turn, without the divisions that a counter would need in every step (an issuer with them: 0.39 us per 128 columns, whatever the tile)
 struct I8Stage { uint32_t s = 0, phase = 0; __device__ __forceinline__ void next(uint32_t count) { if (++s == count) { s = 0; phase ^= 1u; } } };
@@ -98,7 +119,7 @@ template <int CG> __device__ __forceinline__ I8Unit i8_unit(const I8MmaArgs &a, 
     return r;
 }
 
-template <int CG, bool GATHER>
+template <int CG, bool GATHER, bool SPLIT>
 __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const I8MmaArgs a) {
     extern __shared__ uint8_t dyn_smem[];
     __shared__ __align__(8) uint64_t s_bar[2 * I8_STAGES + 5];
@@ -106,7 +127,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
     __shared__ __align__(16) float s_xs[2][I8_N_MAX];
     __shared__ __align__(16) uint32_t s_row[2][I8_N_MAX];
     __shared__ uint32_t s_src[GATHER ? 4 : 1][GATHER ? I8_N_MAX : 1];   // a copying warp's source rows of its unit
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, rank = CG == 2 ? cluster_rank() : 0u;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, part = SPLIT || CG == 2 ? cluster_rank() : 0u, rank = CG == 2 ? part : 0u;   // part: of k, rank: of a pair
     const uint32_t smem_base = (smem_u32(dyn_smem) + 1023u) & ~1023u;
     const uint32_t bar0 = smem_u32(s_bar);
     auto full_bar = [&](uint32_t s) { return bar0 + 8u * s; };
@@ -141,10 +162,10 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
     __syncthreads();
     if constexpr (CG == 2) cluster_sync();
     tc_fence_after();
-    const uint32_t tmem = s_tmem, KB = (a.k + 127u) / 128u;
+    const uint32_t tmem = s_tmem, kb_all = (a.k + 127u) / 128u, kb0 = SPLIT ? kb_all * part / a.split : 0u, KB = SPLIT ? kb_all * (part + 1u) / a.split - kb0 : kb_all;   // this CTA's 128-column blocks
     if (!a.early || warp != 0) griddep_chain();   // early weights are requested while the kernels ahead still run
     const uint32_t total = a.early ? s_total : units();
-    const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
+    const uint32_t first = SPLIT ? blockIdx.x / a.split : blockIdx.x / CG, step = SPLIT ? gridDim.x : gridDim.x / CG;   // SPLIT: one unit
     auto tile_rows = [](uint32_t cnt) { return (cnt + 16u * CG - 1u) / (16u * CG) * 16u; };   // rows of a tile that this CTA holds
     auto filled_bar = [&](uint32_t s) { return CG == 2 ? in_first_cta(full_bar(s)) : full_bar(s); };
 
@@ -158,7 +179,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
                 if (!(ok = i8_wait<CG>(empty_bar(st.s), st.phase ^ 1u, abort_flag, a.err, 1))) break;
                 if (elect_one()) {
                     if (rank == 0) mbar_expect_tx(full_bar(st.s), CG * A_TILE);
-                    i8_load<CG>(smem_base + st.s * stage_bytes, &tm_w, filled_bar(st.s), (int)(kb * 128u), wy);
+                    i8_load<CG>(smem_base + st.s * stage_bytes, &tm_w, filled_bar(st.s), (int)((kb0 + kb) * 128u), wy);
                 }
                 __syncwarp();
             }
@@ -201,7 +222,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
                     if (!(ok = i8_wait<CG>(empty_bar(st.s), st.phase ^ 1u, abort_flag, a.err, 6))) break;
                     if (elect_one()) {
                         if (rank == 0) mbar_expect_tx(full_bar(st.s), CG * boxes * a.box * 128u);
-                        for (uint32_t i = 0; i < boxes; i++) i8_load<CG>(smem_base + st.s * stage_bytes + A_TILE + i * a.box * 128u, &tm_x, filled_bar(st.s), (int)(kb * 128u), y + (int)(i * a.box));
+                        for (uint32_t i = 0; i < boxes; i++) i8_load<CG>(smem_base + st.s * stage_bytes + A_TILE + i * a.box * 128u, &tm_x, filled_bar(st.s), (int)((kb0 + kb) * 128u), y + (int)(i * a.box));
                     }
                     __syncwarp();
                 }
@@ -240,7 +261,15 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
             if (!(ok = i8_wait<CG>(accfull_bar(buf), acc.phase, abort_flag, a.err, 4))) break;
             tc_fence_after();
             const uint32_t taddr = tmem + ((quarter * 32u) << 16) + buf * a.n_cap, ch0 = t.c0 + rank * 128u + quarter * 32u;
-            if (a.packed) {
+            if constexpr (SPLIT) {   // the stages have been read: their memory takes the sums, [row][channel]
+                for (uint32_t c = sub * 16u; c < t.cnt; c += 64u) {
+                    uint32_t v[16];
+                    TMEM_LD16(taddr + c, v, 0);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; i++) asm volatile("st.shared.b32 [%0], %1;" ::"r"(smem_base + ((c + i) * 128u + quarter * 32u + lane) * 4u), "r"(v[i]) : "memory");
+                }
+            } else if (a.packed) {
                 // a thread holds two neighbouring rows of a channel per register pair; the transposing store makes them 16-byte runs of a row's channels
                 uint32_t v[16];
                 const uint32_t part = lane & 3u, piece_ch = ch0 + part * 8u;
@@ -343,6 +372,42 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
             if (ok && behind) pass_on();
         }
     }
+    if constexpr (SPLIT) {
+        // ---------------------------------------------------------------- the parts' sums: every split-th row, two rows of 128 channels at a time per warp
+        if (warp == 0) griddep_wait();   // the one that has not: it reads scales and writes results now
+        __syncwarp();
+        cluster_sync();
+        const uint32_t warps = blockDim.x / 32u, c = (lane & 15u) * 4u;
+        if (first < total) {
+            const I8Unit t = i8_unit<CG>(a, first);
+            const uint32_t ch = t.c0 + c;
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) { const uint32_t n = ch + (i & 3) + (i >> 2) * 64u; w[i] = n < a.n ? __ldg(a.ws + n) : 0.0f; }
+            for (uint32_t j = part + a.split * (warp * 2u + (lane >> 4)); j < t.cnt; j += a.split * warps * 2u) {
+                const float xs = a.xs[t.row0 + j];
+                const uint32_t from = smem_base + (j * 128u + c) * 4u;
+                int sum[8];
+                if (a.split == 2u) i8_sum_parts<2>(from, sum); else if (a.split == 4u) i8_sum_parts<4>(from, sum); else i8_sum_parts<8>(from, sum);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t n = ch + h * 64u;
+                    const size_t at = (size_t)(t.row0 + j) * a.n + n;
+                    float y[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) y[i] = (float)sum[4 * h + i] * (xs * w[4 * h + i]);
+                    if (a.packed) {
+                        if (n < a.n) *reinterpret_cast<uint2 *>(a.y16 + at) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) if (n + i < a.n) { if (a.y16) a.y16[at + i] = (uint16_t)bf16_rne_bits(y[i]); if (a.y32) a.y32[at + i] = y[i]; }
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync();   // the other parts read this one's memory
+    }
     // ---------------------------------------------------------------- teardown
     if (*abort_flag) { for (int i = 0; i < 64; i++) __nanosleep(1000); }   // let copies already issued land before the CTA goes away
     tc_fence_before();
@@ -354,34 +419,45 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
     }
 }
 
-template <int CG, bool GATHER>
+template <int CG, bool GATHER, bool SPLIT>
 static cudaError_t i8_mma_start(const CUtensorMap &w, const CUtensorMap &x, const I8MmaArgs &a, uint32_t grid, cudaStream_t s) {
-    auto kernel = i8_mma_kernel<CG, GATHER>;
+    auto kernel = i8_mma_kernel<CG, GATHER, SPLIT>;
     // set on every call: it belongs to the device's context and costs well under a launch
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)I8_SMEM);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {}; cudaLaunchAttribute at[2];
-    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(i8_threads(GATHER)); cfg.dynamicSmemBytes = I8_SMEM; cfg.stream = s; cfg.attrs = at; cfg.numAttrs = CG;
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(i8_threads(GATHER)); cfg.dynamicSmemBytes = I8_SMEM; cfg.stream = s; cfg.attrs = at; cfg.numAttrs = SPLIT || CG == 2 ? 2 : 1;
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension; at[1].val.clusterDim.x = 2; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension; at[1].val.clusterDim.x = SPLIT ? a.split : CG; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
     return cudaLaunchKernelEx(&cfg, kernel, w, x, a);
 }
 
-// Form and tile of a dense product: the least of rounds * (the slower of a unit's mainloop and drain) + one drain, in us, over tile counts that divide the rows evenly.
-// Per 128 columns, measured with n rows in a tile: one CTA 0.22 + 0.00042 n and at least 0.27, a pair 0.15 + 0.0004 n and at least 0.19; draining a 128 x n accumulator
-// 0.5 + 0.013 n while all SMs store.
-static void i8_dense_form(uint32_t m, uint32_t n, uint32_t k, uint32_t sms, uint32_t *cg, uint32_t *rows) {
-    const float kb = (float)((k + 127u) / 128u);
-    float best = 3.4e38f;
+// Form and tile of a dense product: the least estimate, in us, over tile counts that divide the rows evenly. Measured with r rows in a tile, on L2-resident operands:
+// 128 columns take 0.22 + 0.00042 r and at least 0.26 with one CTA, 0.15 + 0.0004 r and at least 0.19 with a pair, whose start costs 1.4 more; a unit's drain keeps a later one
+// waiting from 0.5 + 0.013 r on and costs 0.2 + 0.008 r where none follows; a split costs 0.9 + 0.35 log2(parts) + 0.014 r. 64 x 4096 x 4096: 10.3 us in one part, 8.7 in two, 7.5 in
+// four; 30 x 512 x 4096: 10.0, 8.1, 6.5, 5.8 in eight; 300 x 4096 x 2048: 7.6 with tiles of 80, 8.2 of 160, 11.0 of 64 (two rounds), 8.8 in pairs.
+struct I8Form { uint32_t cg, rows, split; };
+static I8Form i8_dense_form(uint32_t m, uint32_t n, uint32_t k, uint32_t sms) {
+    const uint32_t kb = (k + 127u) / 128u;
+    I8Form f = {}; float best = 3.4e38f;
     for (uint32_t g = 1; g <= 2; g++) {
         const uint32_t blocks = (n + 128u * g - 1u) / (128u * g), least = (m + I8_N_MAX - 1u) / I8_N_MAX, workers = sms / g;
         for (uint32_t t = least; t < least + 24u && t <= m; t++) {
             const uint32_t r = ((m + t - 1u) / t + 16u * g - 1u) / (16u * g) * (16u * g);
-            const float each = g == 1u ? fmaxf(0.27f, 0.22f + 0.00042f * r) : fmaxf(0.19f, 0.15f + 0.0004f * r), drain = 0.5f + 0.013f * r;
-            const float rounds = ceilf((float)((m + r - 1u) / r) * blocks / workers), cost = rounds * fmaxf(kb * each, drain) + drain;
-            if (cost < best) { best = cost; *cg = g; *rows = r; }
+            const float each = g == 1u ? fmaxf(0.26f, 0.22f + 0.00042f * r) : fmaxf(0.19f, 0.15f + 0.0004f * r);
+            const uint64_t units = (uint64_t)((m + r - 1u) / r) * blocks;
+            const float cost = (float)((units + workers - 1u) / workers) * fmaxf(kb * each, 0.5f + 0.013f * r) + 0.2f + 0.008f * r + (g == 2u ? 1.4f : 0.0f);
+            if (cost < best) { best = cost; f = {g, r, 1u}; }
+            if (g == 2u) continue;
+            uint32_t room = sms;   // clusters of 4 and 8 do not fill the SMs of every group that a cluster has to lie in: 16 of 8 took two rounds
+            for (uint32_t s = 2, lg = 1; s <= 8u && s <= kb; s *= 2u, lg++, room -= sms / 8u) {
+                if (units * s > room) break;
+                const float split = (float)((kb + s - 1u) / s) * each + 0.9f + 0.35f * lg + 0.014f * r;
+                if (split < best) { best = split; f = {1u, r, s}; }
+            }
         }
     }
+    return f;
 }
 
 cudaError_t launch_i8_mma(const OmegaGpuI8Tensor *t, const I8Launch &l, cudaStream_t s) {
@@ -392,9 +468,8 @@ cudaError_t launch_i8_mma(const OmegaGpuI8Tensor *t, const I8Launch &l, cudaStre
     uint32_t cg = 1;
     if (l.tiles) { a.tile_rows = l.tile_rows; a.n_cap = (l.tile_rows + 15u) / 16u * 16u; }   // an expert's tiles: one CTA (gate|up of 4096 tokens: 122 us, 117 - 123 in pairs; down: 80 and 92)
     else {
-        i8_dense_form(l.m, l.n, t->k, sms, &cg, &a.tile_rows);
-        const char *env = getenv("I8_FORM"); if (env) cg = atoi(env) + 1; env = getenv("I8_N"); if (env) a.tile_rows = atoi(env);   // development
-        a.n_cap = a.tile_rows; a.tiles_dense = (l.m + a.tile_rows - 1u) / a.tile_rows;
+        const I8Form f = i8_dense_form(l.m, l.n, t->k, sms);
+        cg = f.cg; a.split = f.split; a.tile_rows = a.n_cap = f.rows; a.tiles_dense = (l.m + f.rows - 1u) / f.rows;
     }
     a.cblocks = (l.n + 128u * cg - 1u) / (128u * cg);
     const uint32_t per_cta = a.n_cap / cg;
@@ -407,9 +482,10 @@ cudaError_t launch_i8_mma(const OmegaGpuI8Tensor *t, const I8Launch &l, cudaStre
     if (!make_tmap_u8(&w, t->w, t->n, t->k, 128) || !make_tmap_u8(&x, l.x, l.x_rows, t->k, a.box, l.x_stride)) return cudaErrorInvalidValue;
     const uint64_t units = (uint64_t)(l.tiles ? l.m : a.tiles_dense) * a.cblocks;
     if (units > 0x7fffffffull) return cudaErrorInvalidValue;
+    if (a.split > 1u) return i8_mma_start<1, false, true>(w, x, a, (uint32_t)units * a.split, s);
     uint32_t grid = (uint32_t)(units * cg < sms ? units * cg : sms); grid -= grid % cg;
-    if (cg == 2u) return i8_mma_start<2, false>(w, x, a, grid, s);
-    return l.xmap ? i8_mma_start<1, true>(w, x, a, grid, s) : i8_mma_start<1, false>(w, x, a, grid, s);
+    if (cg == 2u) return i8_mma_start<2, false, false>(w, x, a, grid, s);
+    return l.xmap ? i8_mma_start<1, true, false>(w, x, a, grid, s) : i8_mma_start<1, false, false>(w, x, a, grid, s);
 }
 
 }  // namespace b200
