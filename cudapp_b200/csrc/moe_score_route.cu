@@ -4,9 +4,12 @@
 //   s_e = softmax(l)_e or 1 / (1 + exp(-l_e));  c_e = s_e + b_e;  rank of a group = sum of its one or two largest c;  picks = topk largest c of the kept groups;
 //   w = s / (sum of the picks' s + 1e-20) * weight_scale.
 //
-// Scores are computed in binary64 and rounded once to f32. Two experts whose c differ by an ulp would else change places with the exponential of the day (about
-// one token in 5000 at 256 experts), and the ids are exact values that a caller compares. The picks are then made on 32-bit keys in the floats' order, which
-// one redux instruction per round reduces.
+// The picks are those of scores computed in binary64 and rounded once to f32: two experts whose c differ by an ulp would else change places with the exponential of the day
+// (about one token in 5000 at 256 experts), and the ids are exact values that a caller compares. A first pass takes f32 scores and looks for the few experts that can
+// be among the picks, by more than the scores' error bound; those, one per lane, get their scores in binary64 and are ranked. Where the f32 scores do not decide which
+// groups are kept, or more than 32 experts are as good as equal, a second pass does it all in binary64. Values are ordered as 32-bit keys, which one redux instruction
+// reduces. 8192 tokens x 256 experts in groups: 14.2 us, bound by instruction issue (about 1100 a token; the 9 MB of memory traffic would take 1.5 us); 17.7 with
+// binary64 scores for every expert. One token: 4.0 us.
 #include <math.h>
 #include "internal.h"
 
@@ -16,24 +19,26 @@ struct RouteArgs {
     const void *logits; const float *bias; uint32_t *ids; float *wts;
     size_t stride;                       // bytes between rows of logits
     uint32_t tokens, experts, topk, groups, kept, rank2, size;   // size = experts / groups
-    int bf16, sigmoid, norm, vec;
+    int bf16, sigmoid, norm, vec, bias_vec;
+    uint32_t magic;                      // e / size = umulhi(e, magic) for e < 1024, size > 1
     float scale;
 };
 
 constexpr uint32_t ROUTE_WARPS = 4;
 constexpr uint32_t KEY_NAN = 1;          // below the key of -infinity; 0 = not to be picked
 __device__ __forceinline__ uint32_t order_key(float v) {   // larger float, larger key; NaN lowest
-    if (v != v) return KEY_NAN;
-    const uint32_t b = __float_as_uint(v + 0.0f);          // -0 becomes +0: they are equal
-    return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+    const uint32_t b = __float_as_uint(v);                 // never -0: scores are not, and a sum is only where both parts are
+    return v != v ? KEY_NAN : b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 __device__ __forceinline__ void push_top2(float v, float &a, float &b) { if (v > a) { b = a; a = v; } else if (v > b) b = v; }
 
 // One warp per token; a lane holds the VPL consecutive experts from lane * VPL, so the lowest lane of equal keys holds the lowest index.
 template <int VPL>
-__global__ void __launch_bounds__(ROUTE_WARPS * 32) score_route_kernel(const RouteArgs a) {
+__global__ void __launch_bounds__(ROUTE_WARPS * 32, VPL <= 8 ? 8 : 2) score_route_kernel(const RouteArgs a) {
     griddep_chain();
-    extern __shared__ float route_sm[];   // [warp][experts], only where groups do not fall on whole lanes
+    extern __shared__ float route_sm[];   // [warp][experts]
+    __shared__ uint64_t s_cand[ROUTE_WARPS][32];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, t = blockIdx.x * ROUTE_WARPS + warp;
     if (t >= a.tokens) return;
     const uint32_t e0 = lane * VPL;
@@ -61,93 +66,209 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) score_route_kernel(const Rou
             l[i] = e >= a.experts ? -INFINITY : a.bf16 ? __uint_as_float((uint32_t) reinterpret_cast<const uint16_t *>(row)[e] << 16) : reinterpret_cast<const float *>(row)[e];
         }
     }
-    float s[VPL];
-    if (a.sigmoid) {
-#pragma unroll
-        for (int i = 0; i < VPL; i++) s[i] = l[i] != l[i] ? 0.0f : (float)(1.0 / (1.0 + exp(-(double)l[i])));
-    } else {
-        float top = -INFINITY;
+    float top = -INFINITY;
+    if (!a.sigmoid) {
 #pragma unroll
         for (int i = 0; i < VPL; i++) top = fmaxf(top, l[i]);   // drops NaN
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        double e[VPL], sum = 0.0;
+    }
+    const int inside = e0 >= a.experts ? 0 : a.experts - e0 < VPL ? (int)(a.experts - e0) : VPL;   // experts of this lane
+    float bias[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; i++) bias[i] = 0.0f;
+    if (a.bias_vec) {
+        if (e0 < a.experts) {
+#pragma unroll
+            for (int i = 0; i < VPL; i += 4) { const float4 b = *reinterpret_cast<const float4 *>(a.bias + e0 + i); bias[i] = b.x; bias[i + 1] = b.y; bias[i + 2] = b.z; bias[i + 3] = b.w; }
+        }
+    } else if (a.bias) {
+#pragma unroll
+        for (int i = 0; i < VPL; i++) if (e0 + i < a.experts) bias[i] = a.bias[e0 + i];
+    }
+    float s[VPL];
+    double sum = 0.0;      // of the softmax
+    uint32_t my_id = 0, my_rank = lane; float my_s = 0.0f;   // a pick and its place
+    float *cs = route_sm + warp * a.experts + e0;   // this lane's values
+    // a score's part in binary64; l == top also where both are +infinity
+    auto score = [&](float v) {
+        if (v != v) return 0.0;
+        if (a.sigmoid) return 1.0 / (1.0 + exp(-(double)v));
+        return v == -INFINITY ? 0.0 : v == top ? 1.0 : exp((double)v - (double)top);
+    };
+#pragma unroll 1
+    for (int exact = 0; exact < 2; exact++) {
+        sum = 0.0;
+        if (exact) {   // two values at a time through shared memory: unrolled, this rare pass would take the registers of the common one
+#pragma unroll
+            for (int i = 0; i < VPL; i++) if (e0 + i < a.experts) cs[i] = l[i];
+            double all = 1.0;
+            if (!a.sigmoid) {
+#pragma unroll 2
+                for (uint32_t i = 0; i < VPL && e0 + i < a.experts; i++) sum += score(cs[i]);
+                for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                all = sum > 0.0 ? sum : 1.0;
+            }
+#pragma unroll 2
+            for (uint32_t i = 0; i < VPL && e0 + i < a.experts; i++) cs[i] = a.sigmoid ? (float)score(cs[i]) : (float)(score(cs[i]) / all);
+#pragma unroll
+            for (int i = 0; i < VPL; i++) s[i] = e0 + i < a.experts ? cs[i] : 0.0f;
+        } else if (a.sigmoid) {
+#pragma unroll
+            for (int i = 0; i < VPL; i++) s[i] = __fdividef(1.0f, 1.0f + __expf(-l[i]));   // NaN stays NaN
+        } else {
+#pragma unroll
+            for (int i = 0; i < VPL; i++) { s[i] = l[i] != l[i] || l[i] == -INFINITY ? 0.0f : l[i] == top ? 1.0f : __expf(l[i] - top); sum += (double)s[i]; }
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const float inv = sum > 0.0 ? (float)(1.0 / sum) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < VPL; i++) s[i] *= inv;
+        }
+        uint32_t key[VPL];
+        float c[VPL];
 #pragma unroll
         for (int i = 0; i < VPL; i++) {
-            e[i] = l[i] != l[i] || l[i] == -INFINITY ? 0.0 : l[i] == top ? 1.0 : exp((double)l[i] - (double)top);   // l == top also where both are +infinity
-            sum += e[i];
+            c[i] = a.sigmoid && !exact ? s[i] + bias[i] : l[i] != l[i] ? NAN : s[i] + bias[i];
+            key[i] = i < inside ? order_key(c[i]) : 0u;
         }
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-#pragma unroll
-        for (int i = 0; i < VPL; i++) s[i] = sum > 0.0 ? (float)(e[i] / sum) : 0.0f;
-    }
-    uint32_t key[VPL];
-    float c[VPL];
-#pragma unroll
-    for (int i = 0; i < VPL; i++) {
-        const uint32_t e = e0 + i;
-        c[i] = a.bias && e < a.experts ? s[i] + a.bias[e] : s[i];
-        if (l[i] != l[i]) c[i] = NAN;
-        key[i] = e < a.experts ? order_key(c[i]) : 0u;
-    }
-    if (a.kept < a.groups) {
-        // rank of group g on lane g
-        float rank = -INFINITY;
-        const uint32_t span = a.size / VPL;   // lanes of a group, where it falls on whole lanes
-        if (a.size % VPL == 0 && (span & (span - 1u)) == 0u) {
-            float x = -INFINITY, y = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < VPL; i++) push_top2(c[i], x, y);   // comparisons with NaN are false: it counts as the lowest
-            for (uint32_t o = 1; o < span; o <<= 1) {
-                const float ox = __shfl_xor_sync(0xffffffffu, x, o), oy = __shfl_xor_sync(0xffffffffu, y, o);
-                push_top2(ox, x, y); push_top2(oy, x, y);
-            }
-            const float r = a.rank2 ? x + y : x;
-            rank = __shfl_sync(0xffffffffu, r, (lane * span) & 31u);
-        } else {
-            float *cs = route_sm + warp * a.experts;
-#pragma unroll
-            for (int i = 0; i < VPL; i++) if (e0 + i < a.experts) cs[e0 + i] = c[i];
-            __syncwarp();
-            if (lane < a.groups) {
+        const float most = a.sigmoid ? 1.0f : sum > 0.0 ? (float)(1.0 / sum) : 1.0f;   // no score is larger
+        bool near = false;   // f32 scores do not decide
+        if (a.kept < a.groups) {
+            // rank of group g on lane g
+            float rank = -INFINITY;
+            const uint32_t span = a.size / VPL;   // lanes of a group, where it falls on whole lanes
+            const bool whole = a.size % VPL == 0 && (span & (span - 1u)) == 0u;
+            if (whole) {
                 float x = -INFINITY, y = -INFINITY;
-                for (uint32_t i = 0; i < a.size; i++) push_top2(cs[lane * a.size + i], x, y);
-                rank = a.rank2 ? x + y : x;
+#pragma unroll
+                for (int i = 0; i < VPL; i++) push_top2(c[i], x, y);   // comparisons with NaN are false: it counts as the lowest
+                for (uint32_t o = 1; o < span; o <<= 1) {
+                    const float ox = __shfl_xor_sync(0xffffffffu, x, o), oy = __shfl_xor_sync(0xffffffffu, y, o);
+                    push_top2(ox, x, y); push_top2(oy, x, y);
+                }
+                const float r = a.rank2 ? x + y : x;
+                rank = __shfl_sync(0xffffffffu, r, (lane * span) & 31u);
+            } else {
+                const float *all = route_sm + warp * a.experts;
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < VPL; i++) if (e0 + i < a.experts) cs[i] = c[i];
+                __syncwarp();
+                if (lane < a.groups) {
+                    float x = -INFINITY, y = -INFINITY;
+                    for (uint32_t i = 0; i < a.size; i++) push_top2(all[lane * a.size + i], x, y);
+                    rank = a.rank2 ? x + y : x;
+                }
+                __syncwarp();
+            }
+            uint32_t gkey = lane < a.groups ? order_key(rank) : 0u, keep = 0, who = 0;
+            for (uint32_t r = 0; r < a.kept; r++) {
+                const uint32_t best = __reduce_max_sync(0xffffffffu, gkey);
+                who = __ffs(__ballot_sync(0xffffffffu, gkey == best)) - 1;
+                keep |= 1u << who;
+                if (lane == who) gkey = 0;
+            }
+            const uint32_t next = __reduce_max_sync(0xffffffffu, gkey);
+            const float in = __shfl_sync(0xffffffffu, rank, who), out = __shfl_sync(0xffffffffu, rank, __ffs(__ballot_sync(0xffffffffu, gkey == next)) - 1);
+            near = !(in - out > 5e-6f * most + 5e-7f * (fabsf(in) + fabsf(out)));   // four f32 scores and the roundings of their sums
+            if (whole) {
+                if (!((keep >> (lane >> (31 - __clz(span)))) & 1u)) {
+#pragma unroll
+                    for (int i = 0; i < VPL; i++) key[i] = 0;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VPL; i++) if (!((keep >> (a.size > 1u ? __umulhi(e0 + i, a.magic) : e0 + i)) & 1u)) key[i] = 0;   // past the experts it is 0 anyway
             }
         }
-        uint32_t gkey = lane < a.groups ? order_key(rank) : 0u, keep = 0;
-        for (uint32_t r = 0; r < a.kept; r++) {
-            const uint32_t best = __reduce_max_sync(0xffffffffu, gkey);
-            const uint32_t who = __ffs(__ballot_sync(0xffffffffu, gkey == best)) - 1;
-            keep |= 1u << who;
-            if (lane == who) gkey = 0;
+        if (!exact) {
+            // Candidates: what is not below the topk-th largest of the lanes' best, which is no more than the topk-th largest of all, by more than two scores' error. Of f32 scores
+            // the exponential of x is off by (2 + 1.173 |x|) 2^-23, quotient and sums by 2 units: less than 2e-5 of a score that is no subnormal, and, as
+            // |x| e^-|x| < 0.4, less than 7e-7 of the largest score.
+            uint32_t m = 0, least = 1;
+#pragma unroll
+            for (int i = 0; i < VPL; i++) m = max(m, key[i]);
+            for (uint32_t r = 0; r < a.topk; r++) {
+                const uint32_t best = __reduce_max_sync(0xffffffffu, m);
+                least = max(best, 1u);   // fewer lanes with experts than that: all of theirs
+                if (m == best) m = 0;
+            }
+            const float edge = key_value(least);
+            if (least > KEY_NAN && fabsf(edge) <= 3.0e38f) least = order_key(edge - (a.bias ? 4e-6f * most + 5e-7f * fabsf(edge) : 1e-4f * edge));
+            uint32_t n = 0;
+#pragma unroll
+            for (int i = 0; i < VPL; i++) {
+                const uint32_t those = __ballot_sync(0xffffffffu, key[i] >= least), at = n + __popc(those & ((1u << lane) - 1u));
+                if (key[i] >= least && at < 32u) s_cand[warp][at] = e0 + i;
+                n += __popc(those);
+            }
+            __syncwarp();
+            if (n <= 32u) {
+                uint64_t mine = 0;
+                if (lane < n) {
+                    const uint32_t e = (uint32_t)s_cand[warp][lane];
+                    const float v = a.bf16 ? __uint_as_float((uint32_t) reinterpret_cast<const uint16_t *>(row)[e] << 16) : reinterpret_cast<const float *>(row)[e];
+                    my_id = e;
+                    my_s = a.sigmoid ? (float)score(v) : (float)(score(v) / (sum > 0.0 ? sum : 1.0));
+                    mine = ((uint64_t)order_key(v != v ? v : a.bias ? my_s + a.bias[e] : my_s) << 32) | ~e;   // ~e: the lowest index of equals first
+                }
+                __syncwarp();
+                if (lane < n) s_cand[warp][lane] = mine;
+                __syncwarp();
+                uint32_t place = 0;
+                for (uint32_t j = 0; j < n; j++) place += s_cand[warp][j] > mine;
+                my_rank = lane < n ? place : 32u;
+                if (!a.sigmoid) {
+                    // the softmax's sum is of f32 exponentials: less than 4e-7 off. Neighbours that this could make equal, or no longer equal, are left to the second pass
+                    __syncwarp();
+                    if (lane < n) s_cand[warp][place] = mine;
+                    __syncwarp();
+                    const uint64_t next = place < a.topk && place + 1u < n ? s_cand[warp][place + 1u] : 0;
+                    if ((uint32_t)(next >> 32) > KEY_NAN) {
+                        const float v = key_value((uint32_t)(mine >> 32)), w = key_value((uint32_t)(next >> 32));
+                        near |= v != w && !(v - w > 1e-6f * (a.bias ? most : my_s) + (a.bias ? 2.4e-7f * fabsf(v) : 0.0f));
+                        // equal as they are: the same logit and bias, or near
+                        if (v == w) {
+                            const uint32_t e = my_id, f = ~(uint32_t)next;
+                            const bool same_l = a.bf16 ? reinterpret_cast<const uint16_t *>(row)[e] == reinterpret_cast<const uint16_t *>(row)[f] : reinterpret_cast<const float *>(row)[e] == reinterpret_cast<const float *>(row)[f];
+                            near |= !(same_l && (!a.bias || a.bias[e] == a.bias[f]));
+                        }
+                    }
+                }
+                if (!__any_sync(0xffffffffu, near)) break;
+                my_rank = lane;
+            }
+            __syncwarp();
+            continue;
         }
+        // each lane's best: key, place, value; the winner of a round looks for its next
+        uint32_t best_key = 0, best_i = 0;
+        auto look = [&]() {
+            best_key = 0; best_i = 0;
 #pragma unroll
-        for (int i = 0; i < VPL; i++) if (e0 + i < a.experts && !((keep >> ((e0 + i) / a.size)) & 1u)) key[i] = 0;
-    }
-    uint32_t my_id = 0; float my_s = 0.0f;
-    uint32_t top = 0;
+            for (int i = 0; i < VPL; i++) if (key[i] > best_key) { best_key = key[i]; best_i = i; }
+        };
+        look();
+        for (uint32_t r = 0; r < a.topk; r++) {
+            const uint32_t best = __reduce_max_sync(0xffffffffu, best_key);
+            const uint32_t who = __ffs(__ballot_sync(0xffffffffu, best_key == best)) - 1;
+            float ws = 0.0f;
+            uint32_t id = 0;
+            if (lane == who) {
 #pragma unroll
-    for (int i = 0; i < VPL; i++) top = max(top, key[i]);
-    for (uint32_t r = 0; r < a.topk; r++) {
-        const uint32_t best = __reduce_max_sync(0xffffffffu, top);
-        const uint32_t who = __ffs(__ballot_sync(0xffffffffu, top == best)) - 1;
-        uint32_t at = 0; float sv = 0.0f;
-#pragma unroll
-        for (int i = VPL - 1; i >= 0; i--) if (key[i] == best) { at = i; sv = s[i]; }
-        if (lane == who) {
-            top = 0;
-#pragma unroll
-            for (int i = 0; i < VPL; i++) { if ((uint32_t)i == at) key[i] = 0; top = max(top, key[i]); }
+                for (int i = 0; i < VPL; i++) if ((uint32_t)i == best_i) { ws = s[i]; key[i] = 0; }
+                id = e0 + best_i;
+                look();
+            }
+            id = __shfl_sync(0xffffffffu, id, who); ws = __shfl_sync(0xffffffffu, ws, who);
+            if (lane == r) { my_id = id; my_s = ws; }
         }
-        const uint32_t id = __shfl_sync(0xffffffffu, e0 + at, who);
-        sv = __shfl_sync(0xffffffffu, sv, who);
-        if (lane == r) { my_id = id; my_s = sv; }
     }
-    float sum = lane < a.topk ? my_s : 0.0f;
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane < a.topk) {
-        a.ids[(size_t)t * a.topk + lane] = my_id;
-        a.wts[(size_t)t * a.topk + lane] = (a.norm ? __fdiv_rn(my_s, sum + 1e-20f) : my_s) * a.scale;
+    const bool pick = my_rank < a.topk;
+    float total = pick ? my_s : 0.0f;
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (pick) {
+        a.ids[(size_t)t * a.topk + my_rank] = my_id;
+        a.wts[(size_t)t * a.topk + my_rank] = (a.norm ? __fdiv_rn(my_s, total + 1e-20f) : my_s) * a.scale;
     }
 }
 
@@ -171,7 +292,8 @@ cudaError_t launch_score_route(const OmegaGpuMoeRouteConfig &c, uint32_t tokens,
     a.bf16 = bf16; a.sigmoid = c.score == OMEGA_GPU_MOE_SCORE_SIGMOID; a.norm = c.norm_topk != 0; a.scale = c.weight_scale;
     const uint32_t vpl = c.experts <= 128 ? 4u : c.experts <= 256 ? 8u : c.experts <= 512 ? 16u : 32u;
     a.vec = ((uintptr_t)logits % 16u) == 0 && a.stride % 16u == 0 && c.experts % vpl == 0;
-    const size_t smem = a.kept < a.groups ? (size_t)ROUTE_WARPS * c.experts * 4 : 0;
+    a.bias_vec = bias && ((uintptr_t)bias % 16u) == 0 && c.experts % vpl == 0; a.magic = a.size > 1u ? 0xffffffffu / a.size + 1u : 0u;
+    const size_t smem = (size_t)ROUTE_WARPS * c.experts * 4;
     const dim3 grid((tokens + ROUTE_WARPS - 1) / ROUTE_WARPS), block(ROUTE_WARPS * 32);
     return vpl == 4u ? launch_chained(score_route_kernel<4>, grid, block, smem, s, a) : vpl == 8u ? launch_chained(score_route_kernel<8>, grid, block, smem, s, a)
          : vpl == 16u ? launch_chained(score_route_kernel<16>, grid, block, smem, s, a) : launch_chained(score_route_kernel<32>, grid, block, smem, s, a);
