@@ -78,7 +78,7 @@ for _n, _t in {"omega_gpu_moe_route_async": (C.POINTER(MoeRouteConfig), _U, _V, 
                "omega_gpu_quant_q8_async": (_U, _U, _V, _I, _U, _V, _V, VP), "omega_gpu_swiglu_q8_async": (_U, _U, _V, _I, _V, _V, VP),
                "omega_gpu_i8_gemm_async": (VP, _U, _V, _U, _V, _V, _V, VP), "omega_gpu_i8_gemm_grouped_async": (VP, _U, _U, _U, _V, _V, _V, _V, _V, _U, _V, _V, _V, VP),
                "omega_gpu_moe_i8_layer_async": (VP, _U, _V, _V, _V, _V, VP), "omega_gpu_moe_i8_layer_q8_async": (VP, _U, _V, _V, _V, _V, _V, VP), "omega_gpu_i8_free": (VP,),
-               "omega_gpu_moe_i8_layer_free": (VP,), "omega_gpu_moe_i8_layer_launches": (VP,)}.items():
+               "omega_gpu_moe_i8_layer_free": (VP,), "omega_gpu_moe_i8_layer_launches": (VP,), "omega_gpu_i8_status": (VP, VP), "omega_gpu_moe_i8_layer_status": (VP, VP)}.items():
     getattr(lib, _n).argtypes = _t
 lib.omega_gpu_i8_free.restype = lib.omega_gpu_moe_i8_layer_free.restype = None
 lib.omega_gpu_moe_i8_layer_launches.restype = C.c_uint32

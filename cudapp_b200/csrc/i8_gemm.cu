@@ -10,11 +10,11 @@
 
 namespace b200 {
 
-constexpr uint32_t I8_MAX_K = 32768;
+constexpr uint32_t I8_MAX_K = 32768, I8_MAX_ROWS = 1u << 30;   // rows: of weights and of one call; row numbers are signed in tensor maps
 
 struct I8Args {
     const int8_t *w, *x; const float *ws, *xs; uint16_t *y16; float *y32;
-    size_t x_stride; uint32_t m, n, k, blocks;        // blocks: channel blocks of one matrix
+    size_t x_stride; uint32_t m, n, k, blocks, experts, x_rows;        // n: channels of one matrix, blocks: its 16-channel blocks
     const uint4 *tiles; const uint32_t *header, *xmap, *ymap;
 };
 
@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(256, 2) i8_rows_kernel(const I8Args a) {
         waited = true;
         if (tile >= a.header[2]) return;
         const uint4 tv = a.tiles[tile];
-        expert = tv.x; row0 = tv.y; rows = row0 + tv.z;
+        expert = min(tv.x, a.experts - 1u); row0 = tv.y; rows = row0 + tv.z;
     }
     const int8_t *w = a.w + (size_t)expert * a.n * a.k;
     const int8_t *w0 = w + (size_t)min(n0 + g, a.n - 1u) * a.k, *w1 = w + (size_t)min(n0 + g + 8u, a.n - 1u) * a.k;
@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(256, 2) i8_rows_kernel(const I8Args a) {
 #pragma unroll
             for (int j = 0; j < NT; j++) {
                 const uint32_t r = row0 + j * 8u + g;
-                x[j] = r < rows ? a.x + (size_t)(a.xmap ? a.xmap[r] : r) * a.x_stride : nullptr;
+                x[j] = r < rows ? a.x + (size_t)(a.xmap ? min(a.xmap[r], a.x_rows - 1u) : r) * a.x_stride : nullptr;
             }
         }
 #pragma unroll
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(256, 2) i8_rows_kernel(const I8Args a) {
     int sum = 0;
 #pragma unroll
     for (int q = 0; q < 8; q++) sum += red[q][ch][tok];
-    const float y = (float)sum * (a.xs[a.xmap ? a.xmap[r] : r] * __ldg(a.ws + (size_t)expert * a.n + n));
+    const float y = (float)sum * (a.xs[a.xmap ? min(a.xmap[r], a.x_rows - 1u) : r] * __ldg(a.ws + (size_t)expert * a.n + n));
     const size_t at = (size_t)(a.ymap ? a.ymap[r] : r) * a.n + n;
     if (a.y32) a.y32[at] = y;
     if (a.y16) a.y16[at] = (uint16_t)bf16_rne_bits(y);
@@ -95,11 +95,18 @@ cudaError_t launch_i8_gemm(const OmegaGpuI8Tensor *t, const I8Launch &l, cudaStr
     const uint32_t most = l.tiles ? l.tile_rows : l.m, nt = most <= 8u ? 1u : 2u;
     if (most > 16u) return launch_i8_mma(t, l, s);   // 4096 x 4096: 16 rows 6.2 us here, 17 rows 6.9 there
     I8Args a = {};
-    a.w = t->w; a.ws = t->s; a.x = l.x; a.xs = l.xs; a.y16 = l.y16; a.y32 = l.y32; a.x_stride = l.x_stride ? l.x_stride : t->k; a.m = l.m; a.n = l.n; a.k = t->k;
+    a.w = t->w; a.ws = t->s; a.x = l.x; a.xs = l.xs; a.y16 = l.y16; a.y32 = l.y32; a.x_stride = l.x_stride ? l.x_stride : t->k; a.m = l.m; a.n = l.n; a.k = t->k; a.experts = t->n / l.n; a.x_rows = l.x_rows;
     a.tiles = (const uint4 *)l.tiles; a.header = l.header; a.xmap = l.xmap; a.ymap = l.ymap; a.blocks = (l.n + 15u) / 16u;
     const uint64_t grid = (uint64_t)a.blocks * (l.tiles ? l.m : 1u);
     if (grid > 0x7fffffffull) return cudaErrorInvalidValue;
     return nt == 1u ? launch_chained(i8_rows_kernel<1>, dim3((uint32_t)grid), dim3(256), 0, s, a) : launch_chained(i8_rows_kernel<2>, dim3((uint32_t)grid), dim3(256), 0, s, a);
+}
+
+int i8_status(const OmegaGpuI8Tensor *t, cudaStream_t s) {
+    uint32_t code = 0;
+    if (!cuda_ok(cudaMemcpyAsync(&code, t->err, 4, cudaMemcpyDeviceToHost, s), "copy i8 status") || !cuda_ok(cudaStreamSynchronize(s), "i8 status")) return OMEGA_GPU_FP8_CHIP_FAIL;
+    if (code) { set_error("i8 product: a bounded wait inside the tensor-core kernel ran out (code %u)", code); st().latched = true; }
+    return (int)code;
 }
 
 }  // namespace b200
@@ -109,7 +116,7 @@ extern "C" {
 
 static int i8_shape(uint32_t n, uint32_t k) {
     if (!n || !k || k % 16u) return OMEGA_GPU_FP8_BAD_ARGS;
-    return k > I8_MAX_K ? OMEGA_GPU_FP8_TOO_LARGE : OMEGA_GPU_FP8_OK;
+    return k > I8_MAX_K || n > I8_MAX_ROWS ? OMEGA_GPU_FP8_TOO_LARGE : OMEGA_GPU_FP8_OK;
 }
 static int i8_scales(const float *s, uint32_t n) {
     for (uint32_t i = 0; i < n; i++) {
@@ -169,6 +176,7 @@ void omega_gpu_i8_free(OmegaGpuI8Tensor *t) {
 
 int omega_gpu_i8_gemm_async(const OmegaGpuI8Tensor *t, uint32_t m, uint64_t x_va, uint32_t x_stride_bytes, uint64_t x_scale_va, uint64_t y_bf16_va, uint64_t y_f32_va, void *stream) {
     if (!t || !m || !x_va || !x_scale_va || (!y_bf16_va && !y_f32_va) || ((x_va | x_stride_bytes | y_bf16_va | y_f32_va) & 15u) || (x_scale_va & 3u)) return OMEGA_GPU_FP8_BAD_ARGS;
+    if (m > I8_MAX_ROWS) return OMEGA_GPU_FP8_TOO_LARGE;
     if (x_stride_bytes && x_stride_bytes < t->k) { set_error("i8 gemm: rows of %u bytes %u bytes apart", t->k, x_stride_bytes); return OMEGA_GPU_FP8_BAD_ARGS; }
     const int ready = async_ready();
     if (ready != OMEGA_GPU_FP8_OK) return ready;
@@ -180,6 +188,7 @@ int omega_gpu_i8_gemm_async(const OmegaGpuI8Tensor *t, uint32_t m, uint64_t x_va
 
 int omega_gpu_i8_gemm(const OmegaGpuI8Tensor *t, uint32_t m, const int8_t *x, const float *x_scale, uint16_t *y16, float *y32) {
     if (!t || !m || !x || !x_scale || (!y16 && !y32)) return OMEGA_GPU_FP8_BAD_ARGS;
+    if (m > I8_MAX_ROWS) return OMEGA_GPU_FP8_TOO_LARGE;
     Lock l;
     if (!dev_open()) return OMEGA_GPU_FP8_CHIP_FAIL;
     const size_t xb = (size_t)m * t->k, yb = (size_t)m * t->n;
@@ -191,13 +200,19 @@ int omega_gpu_i8_gemm(const OmegaGpuI8Tensor *t, uint32_t m, const int8_t *x, co
     bool ok = to_device(dx, x, xb, s) && to_device(ds, x_scale, (size_t)m * 4, s) && cuda_ok(launch_i8_gemm(t, a, s), "i8 gemm launch");
     if (ok && y16) ok = to_host(y16, d16, yb * 2, s);
     if (ok && y32) ok = to_host(y32, d32, yb * 4, s);
-    ok = ok && cuda_ok(cudaStreamSynchronize(s), "i8 gemm");
-    return ok ? OMEGA_GPU_FP8_OK : OMEGA_GPU_FP8_CHIP_FAIL;
+    return ok && i8_status(t, s) == 0 ? OMEGA_GPU_FP8_OK : OMEGA_GPU_FP8_CHIP_FAIL;
+}
+
+int omega_gpu_i8_status(const OmegaGpuI8Tensor *t, void *stream) {
+    if (!t) return OMEGA_GPU_FP8_BAD_ARGS;
+    Lock l;
+    return i8_status(t, (cudaStream_t)stream);
 }
 
 int omega_gpu_i8_gemm_grouped_async(const OmegaGpuI8Tensor *t, uint32_t experts, uint32_t tile_rows, uint32_t max_tiles, uint64_t tiles_va, uint64_t header_va,
                                     uint64_t xmap_va, uint64_t ymap_va, uint64_t x_va, uint32_t x_rows, uint64_t x_scale_va, uint64_t y_bf16_va, uint64_t y_f32_va, void *stream) {
     if (!t || !experts || t->n % experts || !tile_rows || tile_rows > 256 || !max_tiles || !tiles_va || !header_va || !x_va || !x_rows || !x_scale_va || (!y_bf16_va && !y_f32_va)) return OMEGA_GPU_FP8_BAD_ARGS;
+    if (max_tiles > I8_MAX_ROWS || x_rows > I8_MAX_ROWS) return OMEGA_GPU_FP8_TOO_LARGE;
     if (((tiles_va | x_va | y_bf16_va | y_f32_va) & 15u) || ((header_va | xmap_va | ymap_va | x_scale_va) & 3u)) return OMEGA_GPU_FP8_BAD_ARGS;
     const int ready = async_ready();
     if (ready != OMEGA_GPU_FP8_OK) return ready;

@@ -31,10 +31,10 @@ struct I8MmaArgs {
     const float *ws, *xs; uint16_t *y16; float *y32;
     const uint4 *tiles; const uint32_t *header, *xmap, *ymap;
     const int8_t *x; size_t x_stride; uint32_t x_rows;             // GATHER
-    // n: channels of one matrix; n_cap: accumulator columns of a tile; box: rows of one load; packed: bf16 rows of a multiple of 8 channels; lag: of a copying warp's stages, how many stay in flight behind the newest, 0 or 1;
+    // n: channels of one matrix; tiles_most: all tiles of a dense product, the most of a plan; steps: 16 or 32 (pairs) dense rows each; n_cap: accumulator columns of a tile; box: rows of one load; packed: bf16 rows of a multiple of 8 channels; lag: of a copying warp's stages, how many stay in flight behind the newest, 0 or 1;
     // split: CTAs of a unit; once: weights are read by one tile each and need not stay in L2
     // early: the units and their weights are known before the kernels ahead in the stream have completed
-    uint32_t m, n, k, tile_rows, tiles_dense, cblocks, n_cap, stages, tmem_cols, box, packed, lag, early, split, once;
+    uint32_t m, n, k, experts, tiles_most, steps, cblocks, n_cap, stages, tmem_cols, box, packed, lag, early, split, once;
     uint32_t *err;
 };
 
@@ -114,8 +114,11 @@ template <int CG> __device__ __forceinline__ I8Unit i8_unit(const I8MmaArgs &a, 
     const uint32_t t = u / a.cblocks;
     I8Unit r;
     r.c0 = (u - t * a.cblocks) * (128u * CG);
-    if (a.tiles) { const uint4 v = a.tiles[t]; r.expert = v.x; r.row0 = v.y; r.cnt = v.z; }
-    else { r.expert = 0; r.row0 = t * a.tile_rows; r.cnt = min(a.tile_rows, a.m - r.row0); }
+    if (a.tiles) { const uint4 v = a.tiles[t]; r.expert = min(v.x, a.experts - 1u); r.row0 = v.y; r.cnt = min(v.z, a.n_cap); }   // a plan for other calls must not lead out of this one's buffers
+    else {   // 16 or 32 rows more or less, so that any number of tiles divides them evenly
+        r.expert = 0; r.row0 = (uint32_t)((uint64_t)t * a.steps / a.tiles_most) * (16u * CG);
+        r.cnt = min(a.m, (uint32_t)((uint64_t)(t + 1u) * a.steps / a.tiles_most) * (16u * CG)) - r.row0;
+    }
     return r;
 }
 
@@ -138,7 +141,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
     volatile uint32_t *abort_flag = &s_abort;
     const uint32_t stage_bytes = A_TILE + a.n_cap / CG * 128u;
 
-    auto units = [&]() { return *reinterpret_cast<volatile uint32_t *>(a.err) ? 0u : (a.tiles ? a.header[2] : a.tiles_dense) * a.cblocks; };   // after a recorded failure: no work
+    auto units = [&]() { return *reinterpret_cast<volatile uint32_t *>(a.err) ? 0u : (a.tiles ? min(a.header[2], a.tiles_most) : a.tiles_most) * a.cblocks; };   // after a recorded failure: no work
 
     if (threadIdx.x == 0) {
         s_abort = 0;
@@ -238,7 +241,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
             next = i8_unit<CG>(a, u);
             if (et < next.cnt) {
                 const uint32_t r = next.row0 + et;
-                next_xs = a.xs[a.xmap ? a.xmap[r] : r];
+                next_xs = a.xs[a.xmap ? min(a.xmap[r], a.x_rows - 1u) : r];
                 next_row = a.ymap ? a.ymap[r] : r;
             }
 #pragma unroll
@@ -438,24 +441,24 @@ static cudaError_t i8_mma_start(const CUtensorMap &w, const CUtensorMap &x, cons
 // 128 columns take 0.22 + 0.00042 r and at least 0.26 with one CTA, 0.15 + 0.0004 r and at least 0.19 with a pair, whose start costs 1.4 more; a unit's drain keeps a later one
 // waiting from 0.5 + 0.013 r on and costs 0.2 + 0.008 r where none follows; a split costs 0.9 + 0.35 log2(parts) + 0.014 r. 64 x 4096 x 4096: 10.3 us in one part, 8.7 in two, 7.5 in
 // four; 30 x 512 x 4096: 10.0, 8.1, 6.5, 5.8 in eight; 300 x 4096 x 2048: 7.6 with tiles of 80, 8.2 of 160, 11.0 of 64 (two rounds), 8.8 in pairs.
-struct I8Form { uint32_t cg, rows, split; };
+struct I8Form { uint32_t cg, tiles, split; };
 static I8Form i8_dense_form(uint32_t m, uint32_t n, uint32_t k, uint32_t sms) {
     const uint32_t kb = (k + 127u) / 128u;
     I8Form f = {}; float best = 3.4e38f;
     for (uint32_t g = 1; g <= 2; g++) {
-        const uint32_t blocks = (n + 128u * g - 1u) / (128u * g), least = (m + I8_N_MAX - 1u) / I8_N_MAX, workers = sms / g;
-        for (uint32_t t = least; t < least + 24u && t <= m; t++) {
-            const uint32_t r = ((m + t - 1u) / t + 16u * g - 1u) / (16u * g) * (16u * g);
-            const float each = g == 1u ? fmaxf(0.26f, 0.22f + 0.00042f * r) : fmaxf(0.19f, 0.15f + 0.0004f * r);
-            const uint64_t units = (uint64_t)((m + r - 1u) / r) * blocks;
-            const float cost = (float)((units + workers - 1u) / workers) * fmaxf(kb * each, 0.5f + 0.013f * r) + 0.2f + 0.008f * r + (g == 2u ? 1.4f : 0.0f);
-            if (cost < best) { best = cost; f = {g, r, 1u}; }
+        const uint32_t blocks = (n + 128u * g - 1u) / (128u * g), steps = (m + 16u * g - 1u) / (16u * g), most = I8_N_MAX / (16u * g), least = (steps + most - 1u) / most, workers = sms / g;
+        for (uint32_t t = least; t < least + 24u && t <= steps; t++) {
+            const float r = (float)((steps + t - 1u) / t * (16u * g)), mean = fmaxf((float)m / t, 16.0f);   // rows of the longest tile, of all
+            const float each = g == 1u ? fmaxf(0.26f, 0.22f + 0.00042f * mean) : fmaxf(0.19f, 0.15f + 0.0004f * mean);
+            const uint64_t units = (uint64_t)t * blocks;
+            const float cost = (float)((units + workers - 1u) / workers) * fmaxf(kb * each, 0.5f + 0.013f * mean) + 0.2f + 0.008f * r + (g == 2u ? 1.4f : 0.0f);
+            if (cost < best) { best = cost; f = {g, t, 1u}; }
             if (g == 2u) continue;
             uint32_t room = sms;   // clusters of 4 and 8 do not fill the SMs of every group that a cluster has to lie in: 16 of 8 took two rounds
             for (uint32_t s = 2, lg = 1; s <= 8u && s <= kb; s *= 2u, lg++, room -= sms / 8u) {
                 if (units * s > room) break;
                 const float split = (float)((kb + s - 1u) / s) * each + 0.9f + 0.35f * lg + 0.014f * r;
-                if (split < best) { best = split; f = {1u, r, s}; }
+                if (split < best) { best = split; f = {1u, t, s}; }
             }
         }
     }
@@ -466,14 +469,19 @@ cudaError_t launch_i8_mma(const OmegaGpuI8Tensor *t, const I8Launch &l, cudaStre
     const uint32_t sms = st().sm_count ? st().sm_count : 148;
     I8MmaArgs a = {};
     a.ws = t->s; a.xs = l.xs; a.y16 = l.y16; a.y32 = l.y32; a.tiles = (const uint4 *)l.tiles; a.header = l.header; a.xmap = l.xmap; a.ymap = l.ymap;
-    a.m = l.m; a.n = l.n; a.k = t->k; a.err = t->err; a.x = l.x; a.x_stride = l.x_stride ? l.x_stride : t->k; a.x_rows = l.x_rows; a.early = !l.tiles || l.early;
+    a.m = l.m; a.n = l.n; a.k = t->k; a.experts = t->n / l.n; a.err = t->err; a.x = l.x; a.x_stride = l.x_stride ? l.x_stride : t->k; a.x_rows = l.x_rows; a.early = !l.tiles || l.early;
     // Tiles of few rows: hardly any expert has two. 64 tokens through 128 experts, gate|up 53 -> 50 us and down 29 -> 26 us; 4096 tokens in tiles of 256, 125 -> 134 and 78 -> 82.
     a.once = l.tiles && l.tile_rows <= 64u;
     uint32_t cg = 1;
-    if (l.tiles) { a.tile_rows = l.tile_rows; a.n_cap = (l.tile_rows + 15u) / 16u * 16u; }   // an expert's tiles: one CTA (gate|up of 4096 tokens: 122 us, 117 - 123 in pairs; down: 80 and 92)
+    if (l.tiles) {
+        a.tiles_most = l.m;
+        cg = !l.xmap && l.tile_rows >= 128u ? 2u : 1u;   // long tiles in pairs: a layer of 4096 tokens 328 us instead of 334 in a run of many
+        a.n_cap = (l.tile_rows + 16u * cg - 1u) / (16u * cg) * (16u * cg);
+    }
     else {
         const I8Form f = i8_dense_form(l.m, l.n, t->k, sms);
-        cg = f.cg; a.split = f.split; a.tile_rows = a.n_cap = f.rows; a.tiles_dense = (l.m + f.rows - 1u) / f.rows;
+        cg = f.cg; a.split = f.split; a.tiles_most = f.tiles; a.steps = (l.m + 16u * cg - 1u) / (16u * cg);
+        a.n_cap = (a.steps + f.tiles - 1u) / f.tiles * (16u * cg);
     }
     a.cblocks = (l.n + 128u * cg - 1u) / (128u * cg);
     const uint32_t per_cta = a.n_cap / cg;
@@ -484,7 +492,7 @@ cudaError_t launch_i8_mma(const OmegaGpuI8Tensor *t, const I8Launch &l, cudaStre
     a.tmem_cols = 32; while (a.tmem_cols < 2u * a.n_cap) a.tmem_cols *= 2;
     CUtensorMap w, x;
     if (!make_tmap_u8(&w, t->w, t->n, t->k, 128) || !make_tmap_u8(&x, l.x, l.x_rows, t->k, a.box, l.x_stride)) return cudaErrorInvalidValue;
-    const uint64_t units = (uint64_t)(l.tiles ? l.m : a.tiles_dense) * a.cblocks;
+    const uint64_t units = (uint64_t)a.tiles_most * a.cblocks;
     if (units > 0x7fffffffull) return cudaErrorInvalidValue;
     if (a.split > 1u) return i8_mma_start<1, false, true>(w, x, a, (uint32_t)units * a.split, s);
     uint32_t grid = (uint32_t)(units * cg < sms ? units * cg : sms); grid -= grid % cg;

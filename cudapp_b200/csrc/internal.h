@@ -202,6 +202,8 @@ struct I8Launch {
     int early;   // the plan was complete before the launch ahead of this one began
 };
 cudaError_t launch_i8_gemm(const OmegaGpuI8Tensor *t, const I8Launch &a, cudaStream_t s);
+// waits for s; 0, a negative return code, or the positive code of a bounded wait that ran out (the process is latched then)
+int i8_status(const OmegaGpuI8Tensor *t, cudaStream_t s);
 cudaError_t launch_i8_mma(const OmegaGpuI8Tensor *t, const I8Launch &a, cudaStream_t s);   // i8_mma_sm100.cu
 bool layer_forward(OmegaGpuMoeLayer *L, uint32_t tokens, const uint16_t *logits, const uint16_t *x, float *out32, uint16_t *out16, cudaStream_t s,
                    const uint32_t *ids_in = nullptr, const float *wts_in = nullptr);

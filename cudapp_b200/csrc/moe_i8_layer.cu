@@ -187,8 +187,14 @@ int omega_gpu_moe_i8_layer_bf16(OmegaGpuMoeI8Layer *L, uint32_t tokens, const ui
     if (out_f32) ok = ok && to_host(out_f32, L->out32, xb * 2, s);
     if (ids) ok = ok && to_host(ids, L->ids, rb, s);
     if (wts) ok = ok && to_host(wts, L->wts, rb, s);
-    ok = ok && cuda_ok(cudaStreamSynchronize(s), "i8 layer");
-    return ok ? OMEGA_GPU_FP8_OK : OMEGA_GPU_FP8_CHIP_FAIL;
+    return ok && omega_gpu_moe_i8_layer_status(L, s) == 0 ? OMEGA_GPU_FP8_OK : OMEGA_GPU_FP8_CHIP_FAIL;
+}
+
+int omega_gpu_moe_i8_layer_status(OmegaGpuMoeI8Layer *L, void *stream) {
+    if (!L) return OMEGA_GPU_FP8_BAD_ARGS;
+    Lock l;
+    const int rc = i8_status(L->gu, (cudaStream_t)stream);
+    return rc ? rc : i8_status(L->dn, (cudaStream_t)stream);
 }
 
 uint32_t omega_gpu_moe_i8_layer_launches(const OmegaGpuMoeI8Layer *L) { return L ? L->launches : 0; }

@@ -270,13 +270,14 @@ int omega_gpu_moe_router_f32(OmegaGpuMoeRouter *r, uint32_t rows, const float *x
  * 8-bit rows, and the layer made of them. The _async entries open the library's device on first use; the calling thread's current device has to be that one
  * (BAD_ARGS otherwise). */
 
-/* Routing by scores. Per token: score s_e = softmax over the experts or sigmoid of the logit (computed in 64 bits, rounded to f32); selection value
+/* Routing by scores. Per token: score s_e = softmax over the experts or sigmoid of the logit (the picks are those of scores
+ * computed in 64 bits and rounded to f32, the weights within 2^-20 of theirs); selection value
  * c_e = s_e + bias_e (f32; bias f32 [experts] on the device, optional). With 1 < groups and topk_groups < groups, expert e belongs to group
  * e / (experts / groups), a group's rank is the sum of its group_rank (1 or 2) largest c, and the topk_groups groups of largest rank are kept. The topk largest c
  * of the kept groups are picked in descending order; equal values go to the lowest index, of groups and of experts. Weights: s_e of the picks, divided by
  * (their sum + 1e-20) when norm_topk, times weight_scale. A NaN logit has score 0 and is picked behind every other expert of the kept groups (a NaN value
  * counts as the lowest in its group's rank too); a logit of -infinity has score 0, and where every logit is -infinity or NaN all scores are 0. Logits of
- * +infinity share the softmax equally. experts <= 1024, topk <= 32, groups <= 32 and divides experts, group_rank <= experts / groups,
+ * +infinity share the softmax equally. experts <= 1024, topk <= 32, groups <= 32 and a divisor of experts, group_rank <= experts / groups,
  * topk <= topk_groups * (experts / groups); a NaN bias counts as a NaN logit does, but for the score.
  * The ids and weights are what omega_gpu_moe_plan_async and omega_gpu_moe_layer_routed_async take. */
 enum { OMEGA_GPU_MOE_SCORE_SOFTMAX = 0, OMEGA_GPU_MOE_SCORE_SIGMOID = 1 };
@@ -330,6 +331,10 @@ int omega_gpu_i8_gemm(const OmegaGpuI8Tensor *t, uint32_t m, const int8_t *x, co
 int omega_gpu_i8_gemm_grouped_async(const OmegaGpuI8Tensor *t, uint32_t experts, uint32_t tile_rows, uint32_t max_tiles, uint64_t tiles_va, uint64_t header_va,
                                     uint64_t xmap_va, uint64_t ymap_va, uint64_t x_va, uint32_t x_rows, uint64_t x_scale_va, uint64_t y_bf16_va, uint64_t y_f32_va, void *stream);
 
+/* status of the stream-ordered products with a tensor: waits for `stream`; 0, or the code of a bounded wait that ran out inside a kernel (sticky: later products with the
+ * tensor do nothing, and the process is latched, as by the blocking entry) */
+int omega_gpu_i8_status(const OmegaGpuI8Tensor *t, void *stream);
+
 /* ---- one MoE layer with 8-bit integer expert weights: routing by scores, plan, grouped gate|up rounded to bf16, SiLU gate to 8-bit rows, grouped down rounded to
  * bf16, combine in slot order in f32. gate_up: experts x 2I rows of k = hidden (gate rows first, then up rows, per expert); down: experts x hidden rows of k = I; not
  * owned by the layer, which they outlive; several layers may share them. bias f32 [experts] on the host (copied) or null. The layer owns its scratch: calls on one layer are
@@ -345,6 +350,8 @@ int omega_gpu_moe_i8_layer_q8_async(OmegaGpuMoeI8Layer *l, uint32_t tokens, uint
 /* host buffers; ids / wts optional ([tokens][topk]) */
 int omega_gpu_moe_i8_layer_bf16(OmegaGpuMoeI8Layer *l, uint32_t tokens, const uint16_t *logits_bf16, const uint16_t *x_bf16, uint16_t *out_bf16, float *out_f32,
                                 uint32_t *ids, float *wts);
+/* as omega_gpu_i8_status, of the layer's two tensors */
+int omega_gpu_moe_i8_layer_status(OmegaGpuMoeI8Layer *l, void *stream);
 uint32_t omega_gpu_moe_i8_layer_launches(const OmegaGpuMoeI8Layer *l);
 
 /* Measurement aid, no reference counterpart: the FP8 tensor throughput this GPU sustains when nothing has to be loaded (every SM

@@ -82,6 +82,24 @@ def test_route_ties_masks_and_values_that_are_no_numbers(sigmoid, E, groups, kep
             assert not w[1].any() and not w[2].any()
 
 
+@pytest.mark.parametrize("sigmoid", [True, False])
+@pytest.mark.parametrize("biased", [True, False])
+@pytest.mark.parametrize("E,groups,kept", [(256, 8, 4), (128, 1, 0), (60, 4, 2), (600, 1, 0)])
+def test_route_scores_a_unit_in_the_last_place_apart(sigmoid, biased, E, groups, kept):
+    """logits that are neighbours among the floats, that saturate the sigmoid, or whose softmax is subnormal: f32 scores cannot order them, 64 bits can"""
+    rng = np.random.default_rng(E + sigmoid)
+    l = np.empty((10, E), np.float32)
+    for t, (base, step) in enumerate([(0.7, 1), (0.7, 3), (2.5, 1), (-3.0, 2), (16.9, 40), (30.0, 1), (-20.0, 1)]):
+        l[t] = (np.float32(base).view(np.uint32) + rng.permutation(E).astype(np.uint32) * step).view(np.float32)
+    l[7] = rng.normal(-60, 8, E); l[7, 5] = 40.0                             # one expert takes it all
+    l[8] = np.repeat(rng.normal(0, 1, E // 4), 4)[:E]                        # ties in fours
+    l[9] = rng.normal(0, 1e-6, E)
+    bias = (rng.integers(-3, 3, E) * 0.25).astype(np.float32) if biased else None
+    for topk in (1, 6, 32):
+        if topk <= (kept or groups) * (E // groups):
+            check_route(l, bias, E, topk, sigmoid, groups, kept, 2 if groups > 1 else 1)
+
+
 def test_route_strided_rows_on_another_stream():
     import torch
     rng = np.random.default_rng(5)
@@ -254,6 +272,62 @@ def test_product_on_device_rows_a_stride_apart(m, n, k):
     api.lib.omega_gpu_i8_free(t)
 
 
+@pytest.mark.parametrize("m,n,k", [(1100, 4104, 4112), (4136, 2056, 2064), (2049, 4096, 1024), (900, 4090, 3600)])
+def test_large_products(m, n, k):
+    """pairs of CTAs and their ragged ends; the reference in 64 bits on the GPU"""
+    import torch
+    g = torch.Generator(device="cuda"); g.manual_seed(m)
+    x, w = (torch.randint(-128, 128, s, generator=g, dtype=torch.int8, device="cuda") for s in ((m, k), (n, k)))
+    xs, ws = torch.rand(m, generator=g, device="cuda") + 0.5, torch.rand(n, generator=g, device="cuda") + 0.5
+    rc, t = api.i8_upload_dev(n, k, w.data_ptr(), ws.data_ptr()); ok(rc)
+    y16, y32 = torch.full((m + 1, n), 3.0, dtype=torch.bfloat16, device="cuda"), torch.full((m + 1, n), 3.0, device="cuda")
+    ok(api.lib.omega_gpu_i8_gemm_async(t, m, x.data_ptr(), 0, xs.data_ptr(), y16.data_ptr(), 0, here()))
+    ok(api.lib.omega_gpu_i8_gemm_async(t, m, x.data_ptr(), 0, xs.data_ptr(), 0, y32.data_ptr(), here()))
+    assert api.lib.omega_gpu_i8_status(t, here()) == 0
+    want = (x.double() @ w.double().T) * torch.outer(xs.double(), ws.double())
+    assert bool(((y32[:m].double() - want).abs() <= 3 * EPS24 * want.abs()).all()) and torch.equal(y16[:m], y32[:m].bfloat16())
+    assert bool((y16[m] == 3).all()) and bool((y32[m] == 3).all())
+    api.lib.omega_gpu_i8_free(t)
+
+
+@pytest.mark.parametrize("m", [1, 12, 17, 40, 90, 200, 300, 777])
+@pytest.mark.parametrize("n,k", [(8, 64), (136, 528), (100, 256), (264, 4112), (1032, 2048)])
+def test_bf16_rows_are_the_f32_ones_rounded(m, n, k):
+    """each output alone takes a way of its own out of the accumulators"""
+    import torch
+    rng = np.random.default_rng(m + n)
+    x, xs, w, ws = codes(rng, m, k), scales(rng, m), codes(rng, n, k), scales(rng, n)
+    rc, t = api.i8_upload(w, ws); ok(rc)
+    dx, dxs = dev(x), dev(xs)
+    y16, z16, y32 = (torch.full((m + 1, n), 3.0, dtype=d, device="cuda") for d in (torch.bfloat16, torch.bfloat16, torch.float32))
+    ok(api.lib.omega_gpu_i8_gemm_async(t, m, dx.data_ptr(), 0, dxs.data_ptr(), y16.data_ptr(), 0, here()))
+    ok(api.lib.omega_gpu_i8_gemm_async(t, m, dx.data_ptr(), 0, dxs.data_ptr(), z16.data_ptr(), y32.data_ptr(), here()))
+    check_product(y16[:m].cpu().view(torch.int16).numpy().view(np.uint16), y32[:m].cpu().numpy(), ref.gemm(x, xs, w, ws))
+    assert torch.equal(y16[:m], y32[:m].bfloat16()) and torch.equal(z16, y16) and bool((y16[m] == 3).all())
+    api.lib.omega_gpu_i8_free(t)
+
+
+def test_products_on_two_streams_at_once():
+    import torch
+    rng = np.random.default_rng(11)
+    n, k = 512, 1024
+    w, ws = codes(rng, n, k), scales(rng, n)
+    rc, t = api.i8_upload(w, ws); ok(rc)
+    jobs = []
+    for m in (1, 20, 130, 700):
+        x, xs = codes(rng, m, k), scales(rng, m)
+        jobs.append((torch.cuda.Stream(), m, dev(x), dev(xs), torch.zeros((m, n), device="cuda"), ref.gemm(x, xs, w, ws)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, m, x, xs, y, _ in jobs:
+            ok(api.lib.omega_gpu_i8_gemm_async(t, m, x.data_ptr(), 0, xs.data_ptr(), 0, y.data_ptr(), s.cuda_stream))
+    torch.cuda.synchronize()
+    for _, m, _, _, y, want in jobs:
+        assert np.all(np.abs(y.cpu().numpy() - want) <= 3 * EPS24 * np.abs(want))
+    assert api.lib.omega_gpu_i8_status(t, here()) == 0
+    api.lib.omega_gpu_i8_free(t)
+
+
 def make_plan(ids, E, tile_rows):
     import torch
     T, S = ids.shape
@@ -291,6 +365,14 @@ def test_grouped_product(tile_rows, T, S, E, n, k, skew):
     got = y32.cpu().numpy()
     check_product(y16.cpu().view(torch.int16).numpy().view(np.uint16)[:len(order)], got[:len(order)], want[order])
     assert (got[len(order):] == 3).all()
+    # bf16 rows alone, with and without maps
+    z16 = torch.full((R, n), 3.0, dtype=torch.bfloat16, device="cuda")
+    for xm, ym, a, b, rows, f32 in ((0, 0, xo, so, len(order), y32), (p["xmap"].data_ptr(), p["ymap"].data_ptr(), dx, dxs, T, dev(np.where(np.isnan(want), 0, want).astype(np.float32)))):
+        z16.fill_(3.0)
+        ok(api.lib.omega_gpu_i8_gemm_grouped_async(t, E, tile_rows, p["most"], p["tiles"].data_ptr(), p["header"].data_ptr(), xm, ym, a.data_ptr(), rows, b.data_ptr(), z16.data_ptr(), 0, here()))
+        near = (z16.float() - f32).abs() <= (BF16_HALF * (1 + 2 ** -7) + 4 * EPS24) * f32.abs()
+        assert bool(near.all())
+    assert api.lib.omega_gpu_i8_status(t, here()) == 0
     api.lib.omega_gpu_i8_free(t)
 
 
@@ -354,6 +436,7 @@ def test_layer(T, E, H, I, K, groups, kept, rank):
     assert np.array_equal(ids, wids) and np.all(np.abs(w - ww) <= (K + 5) * EPS24 * ww)
     assert np.linalg.norm(o32 - want) <= LAYER_REL * np.linalg.norm(want)
     assert np.all(np.abs(api.bf16_to_f32(o16) - o32) <= BF16_HALF * np.abs(o32))
+    assert api.lib.omega_gpu_moe_i8_layer_status(L.h, here()) == 0
     assert api.lib.omega_gpu_moe_i8_layer_launches(L.h) == 7 + (T * K // E >= 32)             # one more copies the rows into sorted order
     # fewer tokens than the layer has room for: the same rows
     if T > 3:

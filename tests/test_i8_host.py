@@ -61,9 +61,15 @@ def test_upload_and_product_refusals():
     good = [t, 3, V, 0, V, V, 0, 0]
     for at, v in ((0, None), (1, 0), (2, 0), (2, V + 8), (3, 16), (3, 40), (4, 0), (4, V + 2), (5, 0), (5, V + 8), (6, V + 4)):
         assert L.omega_gpu_i8_gemm_async(*[v if i == at else a for i, a in enumerate(good)]) == api.BAD_ARGS, (at, v)
+    assert L.omega_gpu_i8_gemm_async(t, (1 << 30) + 1, V, 0, V, V, 0, 0) == api.TOO_LARGE and api.i8_upload_dev((1 << 30) + 1, 16, V, V)[0] == api.TOO_LARGE
+    assert L.omega_gpu_i8_gemm_grouped_async(t, 4, 16, 5, V, V, 0, 0, V, (1 << 30) + 1, V, V, 0, 0) == api.TOO_LARGE
     good = [t, 4, 16, 5, V, V, 0, 0, V, 3, V, V, 0, 0]
     for at, v in ((0, None), (1, 0), (1, 5), (2, 0), (2, 257), (3, 0), (4, 0), (4, V + 8), (5, 0), (5, V + 2), (6, V + 2), (7, V + 1), (8, 0), (8, V + 4), (9, 0), (10, 0), (11, 0), (12, V + 8)):
         assert L.omega_gpu_i8_gemm_grouped_async(*[v if i == at else a for i, a in enumerate(good)]) == api.BAD_ARGS, (at, v)
+
+
+def test_status_of_nothing():
+    assert L.omega_gpu_i8_status(None, 0) == api.BAD_ARGS and L.omega_gpu_moe_i8_layer_status(None, 0) == api.BAD_ARGS
 
 
 def test_layer_refusals():
