@@ -14,8 +14,7 @@ constexpr uint32_t I8_MAX_K = 32768, I8_MAX_ROWS = 1u << 30;   // rows: of weigh
 
 struct I8Args {
     const int8_t *w, *x; const float *ws, *xs; uint16_t *y16; float *y32;
-    size_t x_stride; uint32_t m, n, k, blocks, experts, x_rows;        // n: channels of one matrix, blocks: its 16-channel blocks
-    const uint4 *tiles; const uint32_t *header, *xmap, *ymap;
+    size_t x_stride; uint32_t m, n, k;
 };
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -23,29 +22,17 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Up to 16 rows: a CTA takes 16 channels and 8 NT activation rows, its eight warps take turns of 128 columns and add their sums up in shared memory. Operands go from memory
-// straight into the fragments: the sum over k may be taken in any order, so a lane's 16 consecutive bytes serve as its parts of two products. Bound by the weights'
-// way from memory: a warp requests those of four turns (4096 columns of the CTA's 16 channels, 64 KB) before it uses the first, and, where they do not depend on a plan,
-// before the kernels ahead in the stream have completed.
+// A few dense rows: a CTA takes 16 channels and all 8 NT activation rows, its eight warps take turns of 128 columns and add their sums up in shared memory. Operands go from
+// memory straight into the fragments: the sum over k may be taken in any order, so a lane's 16 consecutive bytes serve as its parts of two products. Bound by the weights'
+// way from memory: a warp requests those of four turns (4096 columns of the CTA's 16 channels, 64 KB) before it uses the first, and before the kernels ahead in the
+// stream have completed. 1 x 4096 x 4096: 2.9 us, 5.7 TB/s; 16 rows 3.8, 32 rows 5.6 (7.2 on tcgen05, whose set-up and exchange these sizes do not earn back).
 template <int NT>
 __global__ void __launch_bounds__(256, 2) i8_rows_kernel(const I8Args a) {
     __shared__ int red[8][16][8 * NT + 1];
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3u;
-    const uint32_t tile = blockIdx.x / a.blocks, n0 = (blockIdx.x - tile * a.blocks) * 16u;
-    uint32_t row0 = tile * 8u * NT, rows = a.m, expert = 0;
-    bool waited = false;
-    if (a.tiles) {
-        griddep_chain();
-        waited = true;
-        if (tile >= a.header[2]) return;
-        const uint4 tv = a.tiles[tile];
-        expert = min(tv.x, a.experts - 1u); row0 = tv.y; rows = row0 + tv.z;
-    }
-    const int8_t *w = a.w + (size_t)expert * a.n * a.k;
-    const int8_t *w0 = w + (size_t)min(n0 + g, a.n - 1u) * a.k, *w1 = w + (size_t)min(n0 + g + 8u, a.n - 1u) * a.k;
-    const int8_t *x[NT];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3u, n0 = blockIdx.x * 16u;
+    const int8_t *w0 = a.w + (size_t)min(n0 + g, a.n - 1u) * a.k, *w1 = a.w + (size_t)min(n0 + g + 8u, a.n - 1u) * a.k;
     int acc[NT][4] = {};
-    for (uint32_t c0 = warp * 128u; c0 < a.k || !waited; c0 += 4096u) {
+    for (uint32_t c0 = warp * 128u; c0 < a.k || c0 < 1024u; c0 += 4096u) {   // once for every warp: it has to come to the wait
         uint4 u[8], v[8];
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {
@@ -53,21 +40,15 @@ __global__ void __launch_bounds__(256, 2) i8_rows_kernel(const I8Args a) {
             u[i] = v[i] = make_uint4(0, 0, 0, 0);
             if (c < a.k) { u[i] = __ldg(reinterpret_cast<const uint4 *>(w0 + c)); v[i] = __ldg(reinterpret_cast<const uint4 *>(w1 + c)); }
         }
-        if (!waited) { griddep_chain(); waited = true; }
-        if (c0 < 1024u) {
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-                const uint32_t r = row0 + j * 8u + g;
-                x[j] = r < rows ? a.x + (size_t)(a.xmap ? min(a.xmap[r], a.x_rows - 1u) : r) * a.x_stride : nullptr;
-            }
-        }
+        if (c0 < 1024u) griddep_chain();
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {
             const uint32_t c = c0 + (i >> 1) * 1024u + (i & 1u) * 64u + t * 16u;
 #pragma unroll
             for (int j = 0; j < NT; j++) {
+                const uint32_t r = j * 8u + g;
                 uint4 b = make_uint4(0, 0, 0, 0);
-                if (x[j] && c < a.k) b = *reinterpret_cast<const uint4 *>(x[j] + c);
+                if (r < a.m && c < a.k) b = *reinterpret_cast<const uint4 *>(a.x + (size_t)r * a.x_stride + c);
                 mma_s8(acc[j], u[i].x, v[i].x, u[i].y, v[i].y, b.x, b.y);
                 mma_s8(acc[j], u[i].z, v[i].z, u[i].w, v[i].w, b.z, b.w);
             }
@@ -79,27 +60,29 @@ __global__ void __launch_bounds__(256, 2) i8_rows_kernel(const I8Args a) {
         red[warp][g + 8][j * 8 + 2 * t] = acc[j][2]; red[warp][g + 8][j * 8 + 2 * t + 1] = acc[j][3];
     }
     __syncthreads();
-    if (threadIdx.x >= 128u * NT) return;
-    const uint32_t ch = threadIdx.x & 15u, tok = threadIdx.x >> 4, r = row0 + tok, n = n0 + ch;
-    if (r >= rows || n >= a.n) return;
-    int sum = 0;
+    for (uint32_t i = threadIdx.x; i < 128u * NT; i += 256u) {
+        const uint32_t ch = i & 15u, r = i >> 4, n = n0 + ch;
+        if (r >= a.m || n >= a.n) continue;
+        int sum = 0;
 #pragma unroll
-    for (int q = 0; q < 8; q++) sum += red[q][ch][tok];
-    const float y = (float)sum * (a.xs[a.xmap ? min(a.xmap[r], a.x_rows - 1u) : r] * __ldg(a.ws + (size_t)expert * a.n + n));
-    const size_t at = (size_t)(a.ymap ? a.ymap[r] : r) * a.n + n;
-    if (a.y32) a.y32[at] = y;
-    if (a.y16) a.y16[at] = (uint16_t)bf16_rne_bits(y);
+        for (int q = 0; q < 8; q++) sum += red[q][ch][r];
+        const float y = (float)sum * (a.xs[r] * __ldg(a.ws + n));
+        const size_t at = (size_t)r * a.n + n;
+        if (a.y32) a.y32[at] = y;
+        if (a.y16) a.y16[at] = (uint16_t)bf16_rne_bits(y);
+    }
 }
 
 cudaError_t launch_i8_gemm(const OmegaGpuI8Tensor *t, const I8Launch &l, cudaStream_t s) {
-    const uint32_t most = l.tiles ? l.tile_rows : l.m, nt = most <= 8u ? 1u : 2u;
-    if (most > 16u) return launch_i8_mma(t, l, s);   // 4096 x 4096: 16 rows 6.2 us here, 17 rows 6.9 there
+    // Few rows go to the kernel above while its CTAs are resident at once, and up to 8 in any case (8192 x 8192: 8 rows 16.0 us here, 32 rows 23.9 here and 15.3 there). An expert's
+    // few rows do not: a layer's gate|up of 64 tokens takes 82 us here and 50 there, its whole step of one token 29 and 26.
+    const uint32_t blocks = (l.n + 15u) / 16u, sms = st().sm_count ? st().sm_count : 148;
+    if (l.tiles || l.m > 32u || (l.m > 8u && blocks > 2u * sms)) return launch_i8_mma(t, l, s);
     I8Args a = {};
-    a.w = t->w; a.ws = t->s; a.x = l.x; a.xs = l.xs; a.y16 = l.y16; a.y32 = l.y32; a.x_stride = l.x_stride ? l.x_stride : t->k; a.m = l.m; a.n = l.n; a.k = t->k; a.experts = t->n / l.n; a.x_rows = l.x_rows;
-    a.tiles = (const uint4 *)l.tiles; a.header = l.header; a.xmap = l.xmap; a.ymap = l.ymap; a.blocks = (l.n + 15u) / 16u;
-    const uint64_t grid = (uint64_t)a.blocks * (l.tiles ? l.m : 1u);
-    if (grid > 0x7fffffffull) return cudaErrorInvalidValue;
-    return nt == 1u ? launch_chained(i8_rows_kernel<1>, dim3((uint32_t)grid), dim3(256), 0, s, a) : launch_chained(i8_rows_kernel<2>, dim3((uint32_t)grid), dim3(256), 0, s, a);
+    a.w = t->w; a.ws = t->s; a.x = l.x; a.xs = l.xs; a.y16 = l.y16; a.y32 = l.y32; a.x_stride = l.x_stride ? l.x_stride : t->k; a.m = l.m; a.n = l.n; a.k = t->k;
+    const dim3 grid(blocks), block(256);
+    return l.m <= 8u ? launch_chained(i8_rows_kernel<1>, grid, block, 0, s, a) : l.m <= 16u ? launch_chained(i8_rows_kernel<2>, grid, block, 0, s, a)
+         : l.m <= 24u ? launch_chained(i8_rows_kernel<3>, grid, block, 0, s, a) : launch_chained(i8_rows_kernel<4>, grid, block, 0, s, a);
 }
 
 int i8_status(const OmegaGpuI8Tensor *t, cudaStream_t s) {

@@ -439,7 +439,7 @@ static cudaError_t i8_mma_start(const CUtensorMap &w, const CUtensorMap &x, cons
 
 // Form and tile of a dense product: the least estimate, in us, over tile counts that divide the rows evenly. Measured with r rows in a tile, on L2-resident operands:
 // 128 columns take 0.22 + 0.00042 r and at least 0.26 with one CTA, 0.15 + 0.0004 r and at least 0.19 with a pair, whose start costs 1.4 more; a unit's drain keeps a later one
-// waiting from 0.5 + 0.013 r on and costs 0.2 + 0.008 r where none follows; a split costs 0.9 + 0.35 log2(parts) + 0.014 r. 64 x 4096 x 4096: 10.3 us in one part, 8.7 in two, 7.5 in
+// waiting from 0.5 + 0.013 r on and costs 0.2 + 0.008 r where none follows; a split costs 1.4 + 0.4 log2(parts) + 0.014 r. 64 x 4096 x 4096: 10.3 us in one part, 8.7 in two, 7.5 in
 // four; 30 x 512 x 4096: 10.0, 8.1, 6.5, 5.8 in eight; 300 x 4096 x 2048: 7.6 with tiles of 80, 8.2 of 160, 11.0 of 64 (two rounds), 8.8 in pairs.
 struct I8Form { uint32_t cg, tiles, split; };
 static I8Form i8_dense_form(uint32_t m, uint32_t n, uint32_t k, uint32_t sms) {
@@ -457,7 +457,7 @@ static I8Form i8_dense_form(uint32_t m, uint32_t n, uint32_t k, uint32_t sms) {
             uint32_t room = sms;   // clusters of 4 and 8 do not fill the SMs of every group that a cluster has to lie in: 16 of 8 took two rounds
             for (uint32_t s = 2, lg = 1; s <= 8u && s <= kb; s *= 2u, lg++, room -= sms / 8u) {
                 if (units * s > room) break;
-                const float split = (float)((kb + s - 1u) / s) * each + 0.9f + 0.35f * lg + 0.014f * r;
+                const float split = (float)((kb + s - 1u) / s) * each + 1.4f + 0.4f * lg + 0.014f * r;
                 if (split < best) { best = split; f = {1u, t, s}; }
             }
         }
