@@ -190,8 +190,9 @@ bool ffn_shape_ok(uint32_t hidden, uint32_t inter);
 cudaError_t launch_ffn(const void *tm_gu, const void *tm_qx, const void *tm_dn, const void *tm_qa, uint32_t px, uint32_t pa, const FfnLaunch &m, cudaStream_t s, bool pdl);
 // ---- 8-bit integer path
 int score_route_ok(const OmegaGpuMoeRouteConfig *c);   // OK, or BAD_ARGS with the reason
-// stride: bytes between rows of logits, 0 = dense
-cudaError_t launch_score_route(const OmegaGpuMoeRouteConfig &c, uint32_t tokens, const void *logits, int bf16, size_t stride, const float *bias, uint32_t *ids, float *wts, cudaStream_t s);
+// stride: bytes between rows of logits, 0 = dense; plan: of one token, its tiles, maps and the header's first four words are written too (a tile per pick, in the picks' order)
+cudaError_t launch_score_route(const OmegaGpuMoeRouteConfig &c, uint32_t tokens, const void *logits, int bf16, size_t stride, const float *bias, uint32_t *ids, float *wts, cudaStream_t s,
+                               const OmegaGpuMoePlanOut *plan = nullptr);
 bool q8_length_ok(uint32_t n);                          // a row length that the two launchers below take
 cudaError_t launch_norm_q8(uint32_t tokens, uint32_t hidden, float eps, const void *x, int x_bf16, const void *m, int m_bf16, float *h, const float *nw, uint16_t *xn, int8_t *q, float *sc, cudaStream_t s);
 cudaError_t launch_row_q8(uint32_t rows, uint32_t n, size_t stride, const void *x, int x_bf16, int gate, int8_t *q, float *sc, cudaStream_t s);   // gate: silu(x[0 .. n)) * x[n .. 2n)

@@ -93,13 +93,14 @@ static int i8_layer_run(OmegaGpuMoeI8Layer *L, uint32_t tokens, const uint16_t *
     up.n = 2u * I; up.x = sorted ? L->sq : q; up.xs = sorted ? L->ss : qs; up.x_rows = sorted ? R : tokens; up.xmap = sorted ? nullptr : L->xmap; up.y16 = L->gu16;   // sorted row p = x[xmap[p]] against its expert's 2I x H matrix
     dn.n = H; dn.x = L->aq; dn.xs = L->as; dn.x_rows = R; dn.ymap = L->ymap; dn.y16 = L->dn16;          // result of sorted row p to row ymap[p] = token * K + slot
     up.early = sorted; dn.early = 1;
-    const bool ok = cuda_ok(launch_score_route(L->route, tokens, logits, 1, 0, L->bias, L->ids, L->wts, s), "route launch") &&
-                    cuda_ok(launch_plan(tokens, K, E, K, tr, L->ids, o, s, L->scratch, L->scratch_words), "plan launch") &&
+    // one token's plan is its picks, and the routing writes it (25.8 -> 23 us for such a step)
+    const bool ok = cuda_ok(launch_score_route(L->route, tokens, logits, 1, 0, L->bias, L->ids, L->wts, s, &o), "route launch") &&
+                    (tokens == 1u || cuda_ok(launch_plan(tokens, K, E, K, tr, L->ids, o, s, L->scratch, L->scratch_words), "plan launch")) &&
                     (!sorted || cuda_ok(launch_chained(sort_rows_kernel, dim3((R + 7u) / 8u), dim3(256), 0, s, R, H, L->xmap, q, qs, L->sq, L->ss), "sort rows launch")) &&
                     cuda_ok(launch_i8_gemm(L->gu, up, s), "gate|up launch") &&
                     cuda_ok(launch_row_q8(R, I, 0, L->gu16, 1, 1, L->aq, L->as, s), "swiglu q8 launch") && cuda_ok(launch_i8_gemm(L->dn, dn, s), "down launch") &&
                     cuda_ok(launch_chained(combine16_kernel, dim3(tokens), dim3(H <= 1024u ? 128 : 256), 0, s, tokens, K, H, L->wts, L->dn16, out32, out16), "combine launch");
-    L->launches = (sorted ? 6u : 5u) + plan_launch_count(R, E, L->scratch, L->scratch_words, o);
+    L->launches = (sorted ? 6u : 5u) + (tokens == 1u ? 0u : plan_launch_count(R, E, L->scratch, L->scratch_words, o));
     return ok ? OMEGA_GPU_FP8_OK : OMEGA_GPU_FP8_CHIP_FAIL;
 }
 }  // namespace b200

@@ -20,6 +20,7 @@ struct RouteArgs {
     size_t stride;                       // bytes between rows of logits
     uint32_t tokens, experts, topk, groups, kept, rank2, size;   // size = experts / groups
     int bf16, sigmoid, norm, vec, bias_vec;
+    uint4 *tiles; uint32_t *header, *xmap, *ymap;   // one token: its routing plan as well, or null
     uint32_t magic;                      // e / size = umulhi(e, magic) for e < 1024, size > 1
     float scale;
 };
@@ -269,7 +270,13 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, VPL <= 8 ? 8 : 2) score_rout
     if (pick) {
         a.ids[(size_t)t * a.topk + my_rank] = my_id;
         a.wts[(size_t)t * a.topk + my_rank] = (a.norm ? __fdiv_rn(my_s, total + 1e-20f) : my_s) * a.scale;
+        if (a.tiles) {   // every pick is a tile of one row, in the picks' order
+            a.tiles[my_rank] = make_uint4(my_id, my_rank, 1u, my_rank);
+            a.xmap[my_rank] = 0; a.ymap[my_rank] = my_rank;
+            if (my_rank < 4u) a.header[my_rank] = my_rank < 3u ? a.topk : 0u;
+        }
     }
+    if (a.tiles && lane < 4u && a.topk <= lane) a.header[lane] = lane < 3u ? a.topk : 0u;   // fewer than four picks
 }
 
 static int route_check(const OmegaGpuMoeRouteConfig *c) {
@@ -283,8 +290,10 @@ static int route_check(const OmegaGpuMoeRouteConfig *c) {
 }
 int score_route_ok(const OmegaGpuMoeRouteConfig *c) { return route_check(c); }
 
-cudaError_t launch_score_route(const OmegaGpuMoeRouteConfig &c, uint32_t tokens, const void *logits, int bf16, size_t stride, const float *bias, uint32_t *ids, float *wts, cudaStream_t s) {
+cudaError_t launch_score_route(const OmegaGpuMoeRouteConfig &c, uint32_t tokens, const void *logits, int bf16, size_t stride, const float *bias, uint32_t *ids, float *wts, cudaStream_t s,
+                               const OmegaGpuMoePlanOut *plan) {
     RouteArgs a = {};
+    if (plan && tokens == 1u) { a.tiles = (uint4 *)(uintptr_t)plan->tiles_va; a.header = (uint32_t *)(uintptr_t)plan->header_va; a.xmap = (uint32_t *)(uintptr_t)plan->xmap_va; a.ymap = (uint32_t *)(uintptr_t)plan->ymap_va; }
     const uint32_t elem = bf16 ? 2u : 4u;
     a.logits = logits; a.bias = bias; a.ids = ids; a.wts = wts; a.stride = stride ? stride : (size_t)c.experts * elem;
     a.tokens = tokens; a.experts = c.experts; a.topk = c.topk; a.groups = c.groups ? c.groups : 1u; a.kept = c.topk_groups ? c.topk_groups : a.groups;
