@@ -53,7 +53,6 @@ __global__ void __launch_bounds__(256) sort_rows_kernel(uint32_t rows, uint32_t 
     if (lane == 0) qs_out[p] = qs[src];
 }
 
-constexpr uint32_t I8_SORT_ROWS = 32;   // average rows of an expert from which they are sorted
 static size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 }  // namespace b200
@@ -71,15 +70,17 @@ struct OmegaGpuMoeI8Layer {
 };
 
 namespace b200 {
-// Rows per tile: about twice an expert's average, so that most experts are one tile, which reads their weights once; the tensor cores' time goes by the rows that are there.
+// Rows per tile: an expert's average and half of it again, so that most experts are one tile, which reads their weights once, and a tile leaves the pipeline its stages; the
+// longest where that is more than 96. Measured, 128 experts of 2048 x 768 with an uneven load, us: 512 tokens 147 / 134 / 140 / 150 with 32 / 64 / 96 / 128 rows; 1024 tokens
+// 163 / 160 / 171 / 167 with 64 / 96 / 128 / 256; 2048 tokens 222 / 221 / 211 / 207 with 96 / 128 / 192 / 256.
 static uint32_t i8_tile_rows(uint32_t picks, uint32_t experts) {
-    const uint32_t rows = (2u * picks / experts + 31u) / 32u * 32u;
-    return rows < 32u ? 32u : rows > 256u ? 256u : rows;
+    const uint32_t rows = (3u * (picks / experts) / 2u + 31u) / 32u * 32u;
+    return rows < 32u ? 32u : rows > 96u ? 256u : rows;
 }
-// Rows are copied into sorted order first where experts have many of them: the product then fetches a tile's rows by TMA, which costs less than their copies through the
-// map once a row is used by several channel blocks of a long tile. Measured, gate|up of 128 experts x 1536 x 2048: 64 tokens 53 us either way, 4096 tokens 122 us
-// and 12 for the copies against 216.
-static bool i8_sorted(uint32_t picks, uint32_t experts) { return picks / experts >= I8_SORT_ROWS; }
+// Rows are copied into sorted order first where tiles are long: the product then fetches a tile's rows by TMA, which costs less than their copies through the
+// map once a row is used by several channel blocks of a long tile. Measured: 512 tokens (32 rows an expert) 129.6 us unsorted, 133.7 sorted, 1024 tokens 169.8 and 171.2;
+// gate|up alone of 4096 tokens 122 us and 14 for the copies against 216.
+static bool i8_sorted(uint32_t picks, uint32_t experts) { return i8_tile_rows(picks, experts) == 256u; }
 static uint32_t i8_max_tiles(uint32_t picks, uint32_t experts, uint32_t tile_rows) { return picks / tile_rows + (experts < picks ? experts : picks); }
 
 static int i8_layer_run(OmegaGpuMoeI8Layer *L, uint32_t tokens, const uint16_t *logits, const int8_t *q, const float *qs, float *out32, uint16_t *out16, cudaStream_t s) {

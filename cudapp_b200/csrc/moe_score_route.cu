@@ -25,7 +25,7 @@ struct RouteArgs {
     float scale;
 };
 
-constexpr uint32_t ROUTE_WARPS = 4;
+constexpr uint32_t ROUTE_WARPS = 4, ROUTE_MOST_TOKENS = 1u << 30;
 constexpr uint32_t KEY_NAN = 1;          // below the key of -infinity; 0 = not to be picked
 __device__ __forceinline__ uint32_t order_key(float v) {   // larger float, larger key; NaN lowest
     const uint32_t b = __float_as_uint(v);                 // never -0: scores are not, and a sum is only where both parts are
@@ -320,6 +320,7 @@ int omega_gpu_moe_route_async(const OmegaGpuMoeRouteConfig *cfg, uint32_t tokens
     const uint32_t elem = logits_bf16 ? 2u : 4u;
     if (!tokens || !logits_va || !ids_va || !wts_va || ((ids_va | wts_va | bias_va) & 3u) || logits_va % elem) return OMEGA_GPU_FP8_BAD_ARGS;
     if (logits_stride_bytes && (logits_stride_bytes % elem || logits_stride_bytes < cfg->experts * elem)) { set_error("route: rows of logits %u bytes apart", logits_stride_bytes); return OMEGA_GPU_FP8_BAD_ARGS; }
+    if (tokens > ROUTE_MOST_TOKENS) return OMEGA_GPU_FP8_TOO_LARGE;
     const int ready = async_ready();
     if (ready != OMEGA_GPU_FP8_OK) return ready;
     return cuda_ok(launch_score_route(*cfg, tokens, (const void *)(uintptr_t)logits_va, logits_bf16 != 0, logits_stride_bytes, (const float *)(uintptr_t)bias_va, (uint32_t *)(uintptr_t)ids_va,
@@ -330,6 +331,7 @@ int omega_gpu_moe_route(const OmegaGpuMoeRouteConfig *cfg, uint32_t tokens, cons
     const int rc = route_check(cfg);
     if (rc != OMEGA_GPU_FP8_OK) return rc;
     if (!tokens || !logits || !ids || !wts) return OMEGA_GPU_FP8_BAD_ARGS;
+    if (tokens > ROUTE_MOST_TOKENS) return OMEGA_GPU_FP8_TOO_LARGE;
     Lock l;
     if (!dev_open()) return OMEGA_GPU_FP8_CHIP_FAIL;
     const size_t lb = (size_t)tokens * cfg->experts * (logits_bf16 ? 2 : 4), ib = (size_t)tokens * cfg->topk * 4, bb = (size_t)cfg->experts * 4;

@@ -12,7 +12,7 @@
 
 namespace b200 {
 
-constexpr uint32_t Q8_INF = 0x7f800000u, Q8_MOST = 16384;
+constexpr uint32_t Q8_INF = 0x7f800000u, Q8_MOST = 16384, Q8_MOST_ROWS = 1u << 30;
 
 __device__ __forceinline__ void load8(const uint16_t *p, float (&v)[8]) {
     const uint4 w = *reinterpret_cast<const uint4 *>(p);
@@ -223,6 +223,7 @@ int omega_gpu_residual_norm_q8_async(uint32_t tokens, uint32_t hidden, float eps
                                      uint64_t norm_w_va, uint64_t xn_bf16_va, uint64_t q_va, uint64_t s_va, void *stream) {
     if (!tokens || !x16_va == !h_in_va || !q_va || !s_va || !(eps >= 0.0f) || ((x16_va | m_va | h_in_va | h_va | norm_w_va | xn_bf16_va | q_va) & 15u) || (s_va & 3u)) return OMEGA_GPU_FP8_BAD_ARGS;
     if (!q8_length_ok(hidden)) return OMEGA_GPU_FP8_BAD_ARGS;
+    if (tokens > Q8_MOST_ROWS) return OMEGA_GPU_FP8_TOO_LARGE;
     const int ready = async_ready();
     if (ready != OMEGA_GPU_FP8_OK) return ready;
     return cuda_ok(launch_norm_q8(tokens, hidden, eps, (const void *)(uintptr_t)(x16_va ? x16_va : h_in_va), x16_va != 0, (const void *)(uintptr_t)m_va, m_bf16 != 0, (float *)(uintptr_t)h_va,
@@ -233,6 +234,7 @@ int omega_gpu_residual_norm_q8_async(uint32_t tokens, uint32_t hidden, float eps
 int omega_gpu_quant_q8_async(uint32_t rows, uint32_t k, uint64_t x_va, int x_bf16, uint32_t x_stride_bytes, uint64_t q_va, uint64_t s_va, void *stream) {
     if (!rows || !x_va || !q_va || !s_va || ((x_va | q_va | x_stride_bytes) & 15u) || (s_va & 3u)) return OMEGA_GPU_FP8_BAD_ARGS;
     if (!q8_length_ok(k) || (x_stride_bytes && x_stride_bytes < k * (x_bf16 ? 2u : 4u))) return OMEGA_GPU_FP8_BAD_ARGS;
+    if (rows > Q8_MOST_ROWS) return OMEGA_GPU_FP8_TOO_LARGE;
     const int ready = async_ready();
     if (ready != OMEGA_GPU_FP8_OK) return ready;
     return cuda_ok(launch_row_q8(rows, k, x_stride_bytes, (const void *)(uintptr_t)x_va, x_bf16 != 0, 0, (int8_t *)(uintptr_t)q_va, (float *)(uintptr_t)s_va, (cudaStream_t)stream), "quant q8 launch")
@@ -242,6 +244,7 @@ int omega_gpu_quant_q8_async(uint32_t rows, uint32_t k, uint64_t x_va, int x_bf1
 int omega_gpu_swiglu_q8_async(uint32_t rows, uint32_t inter, uint64_t gu_va, int gu_bf16, uint64_t q_va, uint64_t s_va, void *stream) {
     if (!rows || !gu_va || !q_va || !s_va || ((gu_va | q_va) & 15u) || (s_va & 3u)) return OMEGA_GPU_FP8_BAD_ARGS;
     if (!q8_length_ok(inter)) return OMEGA_GPU_FP8_BAD_ARGS;
+    if (rows > Q8_MOST_ROWS) return OMEGA_GPU_FP8_TOO_LARGE;
     const int ready = async_ready();
     if (ready != OMEGA_GPU_FP8_OK) return ready;
     return cuda_ok(launch_row_q8(rows, inter, 0, (const void *)(uintptr_t)gu_va, gu_bf16 != 0, 1, (int8_t *)(uintptr_t)q_va, (float *)(uintptr_t)s_va, (cudaStream_t)stream), "swiglu q8 launch")
@@ -250,6 +253,7 @@ int omega_gpu_swiglu_q8_async(uint32_t rows, uint32_t inter, uint64_t gu_va, int
 
 int omega_gpu_residual_norm_q8_f32(uint32_t tokens, uint32_t hidden, float eps, const float *x, const float *m, const float *norm_w, float *h, int8_t *q, float *sc) {
     if (!tokens || !x || !q || !sc || !(eps >= 0.0f) || !q8_length_ok(hidden)) return OMEGA_GPU_FP8_BAD_ARGS;
+    if (tokens > Q8_MOST_ROWS) return OMEGA_GPU_FP8_TOO_LARGE;
     Lock l;
     if (!dev_open()) return OMEGA_GPU_FP8_CHIP_FAIL;
     const size_t qb = (size_t)tokens * hidden, xb = qb * 4, wb = (size_t)hidden * 4, sb = (size_t)tokens * 4;
@@ -265,6 +269,7 @@ int omega_gpu_residual_norm_q8_f32(uint32_t tokens, uint32_t hidden, float eps, 
 
 int omega_gpu_swiglu_q8_f32(uint32_t rows, uint32_t inter, const float *gu, int8_t *q, float *sc) {
     if (!rows || !gu || !q || !sc || !q8_length_ok(inter)) return OMEGA_GPU_FP8_BAD_ARGS;
+    if (rows > Q8_MOST_ROWS) return OMEGA_GPU_FP8_TOO_LARGE;
     Lock l;
     if (!dev_open()) return OMEGA_GPU_FP8_CHIP_FAIL;
     const size_t qb = (size_t)rows * inter, gb = qb * 8, sb = (size_t)rows * 4;

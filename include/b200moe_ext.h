@@ -268,7 +268,7 @@ int omega_gpu_moe_router_f32(OmegaGpuMoeRouter *r, uint32_t rows, const float *x
 /* ---- 8-bit integer path: rows and weights as signed 8-bit codes, one f32 scale for each row (token) and each weight row (channel). No counterpart in the
  * reference. What a model quantised this way needs of an expert layer: routing by scores, residual + RMSNorm to 8-bit rows, the product, the SiLU gate to
  * 8-bit rows, and the layer made of them. The _async entries open the library's device on first use; the calling thread's current device has to be that one
- * (BAD_ARGS otherwise). */
+ * (BAD_ARGS otherwise). At most 2^30 rows, of tokens or of weights, per call (TOO_LARGE). */
 
 /* Routing by scores. Per token: score s_e = softmax over the experts or sigmoid of the logit (the picks are those of scores
  * computed in 64 bits and rounded to f32, the weights within 2^-20 of theirs); selection value

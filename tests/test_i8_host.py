@@ -68,6 +68,13 @@ def test_upload_and_product_refusals():
         assert L.omega_gpu_i8_gemm_grouped_async(*[v if i == at else a for i, a in enumerate(good)]) == api.BAD_ARGS, (at, v)
 
 
+def test_too_many_rows():
+    many = (1 << 30) + 1
+    assert L.omega_gpu_moe_route_async(cfg(), many, V, 0, 0, 0, V, V, 0) == api.TOO_LARGE
+    assert L.omega_gpu_residual_norm_q8_async(many, 64, 1e-6, V, 0, 0, 0, 0, 0, 0, V, V, 0) == api.TOO_LARGE
+    assert L.omega_gpu_quant_q8_async(many, 64, V, 1, 0, V, V, 0) == api.TOO_LARGE and L.omega_gpu_swiglu_q8_async(many, 64, V, 1, V, V, 0) == api.TOO_LARGE
+
+
 def test_status_of_nothing():
     assert L.omega_gpu_i8_status(None, 0) == api.BAD_ARGS and L.omega_gpu_moe_i8_layer_status(None, 0) == api.BAD_ARGS
 
