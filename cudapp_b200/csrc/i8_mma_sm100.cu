@@ -13,10 +13,9 @@
 // rows over the cluster. Integer sums: the result is the same, whatever the split.
 //
 // Warps: 0 weights (TMA), 1 MMA issuer (of a pair's first CTA), 2 TMEM, 3 rows (TMA), 4 - 19 epilogue,
-// GATHER 20 - 23 row copies. Every mbarrier wait is bounded; on expiry the kernel records a code in *err, lets its own copies land, frees its TMEM and returns, and
-// later launches on the tensor do nothing.
+// GATHER 20 - 23 row copies. KPS: blocks of 128 columns in a stage of the ring. Every mbarrier wait is bounded; on expiry the kernel
+// records a code in *err, lets its own copies land, frees its TMEM and returns, and later launches on the tensor do nothing.
 #include <math.h>
-#include <stdlib.h>
 #include "internal.h"
 #include "mma_common.cuh"
 
@@ -26,12 +25,14 @@ constexpr uint32_t I8_EPI = 16, I8_STAGES = 12, I8_N_MAX = 256;   // epilogue wa
 constexpr uint32_t i8_threads(bool gather) { return 128 + 32 * I8_EPI + (gather ? 128 : 0); }
 constexpr uint32_t I8_OUT_ROW = 80, I8_OUT = 16 * I8_OUT_ROW;     // an epilogue warp's 16 result rows of 32 bf16 channels; 80 bytes apart: neither side meets a bank twice
 constexpr size_t I8_SMEM = 214 * 1024;                            // dynamic shared memory of every form: stages, result rows, alignment
+constexpr uint32_t I8_ROOM = (uint32_t)I8_SMEM - 1024u - I8_EPI * I8_OUT;   // the stages' part
 
 struct I8MmaArgs {
     const float *ws, *xs; uint16_t *y16; float *y32;
     const uint4 *tiles; const uint32_t *header, *xmap, *ymap;
     const int8_t *x; size_t x_stride; uint32_t x_rows;             // GATHER
-    // n: channels of one matrix; tiles_most: all tiles of a dense product, the most of a plan; steps: 16 or 32 (pairs) dense rows each; n_cap: accumulator columns of a tile; box: rows of one load; packed: bf16 rows of a multiple of 8 channels; lag: of a copying warp's stages, how many stay in flight behind the newest, 0 or 1;
+    // n: channels of one matrix; tiles_most: all tiles of a dense product, the most of a plan; steps: 16 or 32 (pairs) dense rows each; n_cap: accumulator columns of a tile;
+    // box: rows of one load; packed: bf16 rows of a multiple of 8 channels; lag: of a copying warp's stages, how many stay in flight behind the newest, 0 or 1;
     // split: CTAs of a unit; once: weights are read by one tile each and need not stay in L2
     // early: the units and their weights are known before the kernels ahead in the stream have completed
     uint32_t m, n, k, experts, tiles_most, steps, cblocks, n_cap, stages, tmem_cols, box, packed, lag, early, split, once;
@@ -50,14 +51,16 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) { asm volatile
 // the bounded wait of mma_common.cuh, seeing what the other CTA of a pair released
 template <int CG> __device__ __forceinline__ bool i8_wait(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag, uint32_t *err, uint32_t code) {
     if constexpr (CG == 1) return mbar_wait(bar, parity, abort_flag, err, code);
-    for (uint32_t i = 0; i < SPIN_LIMIT; i++) {
-        uint32_t ok;
-        asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-        if (ok) return true;
-        if ((i & 255u) == 255u && *abort_flag) return false;
+    else {
+        for (uint32_t i = 0; i < SPIN_LIMIT; i++) {
+            uint32_t ok;
+            asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+            if (ok) return true;
+            if ((i & 255u) == 255u && *abort_flag) return false;
+        }
+        *abort_flag = 1; atomicCAS(err, 0u, code);
+        return false;
     }
-    *abort_flag = 1; atomicCAS(err, 0u, code);
-    return false;
 }
 template <int CG> __device__ __forceinline__ void i8_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
     if constexpr (CG == 1) tma_load_2d(dst, map, bar, x, y);
@@ -122,7 +125,7 @@ template <int CG> __device__ __forceinline__ I8Unit i8_unit(const I8MmaArgs &a, 
     return r;
 }
 
-template <int CG, bool GATHER, bool SPLIT>
+template <int CG, bool GATHER, bool SPLIT, int KPS>
 __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const I8MmaArgs a) {
     extern __shared__ uint8_t dyn_smem[];
     __shared__ __align__(8) uint64_t s_bar[2 * I8_STAGES + 5];
@@ -139,7 +142,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
     auto accempty_bar = [&](uint32_t b) { return bar0 + 8u * (2 * I8_STAGES + 2 + b); };
     const uint32_t all_bar = bar0 + 8u * (2 * I8_STAGES + 4);   // every epilogue warp; not bar.sync, which would wait for a warp that gave up
     volatile uint32_t *abort_flag = &s_abort;
-    const uint32_t stage_bytes = A_TILE + a.n_cap / CG * 128u;
+    const uint32_t x_tile = a.n_cap / CG * 128u, stage_bytes = KPS * (A_TILE + x_tile);   // KPS weight tiles, then KPS tiles of rows
 
     auto units = [&]() { return *reinterpret_cast<volatile uint32_t *>(a.err) ? 0u : (a.tiles ? min(a.header[2], a.tiles_most) : a.tiles_most) * a.cblocks; };   // after a recorded failure: no work
 
@@ -165,7 +168,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
     __syncthreads();
     if constexpr (CG == 2) cluster_sync();
     tc_fence_after();
-    const uint32_t tmem = s_tmem, kb_all = (a.k + 127u) / 128u, kb0 = SPLIT ? kb_all * part / a.split : 0u, KB = SPLIT ? kb_all * (part + 1u) / a.split - kb0 : kb_all;   // this CTA's 128-column blocks
+    const uint32_t tmem = s_tmem, kb_all = (a.k + 128u * KPS - 1u) / (128u * KPS), kb0 = SPLIT ? kb_all * part / a.split : 0u, KB = SPLIT ? kb_all * (part + 1u) / a.split - kb0 : kb_all;   // this CTA's stages' columns
     if (!a.early || warp != 0) griddep_chain();   // early weights are requested while the kernels ahead still run
     const uint32_t total = a.early ? s_total : units();
     const uint32_t first = SPLIT ? blockIdx.x / a.split : blockIdx.x / CG, step = SPLIT ? gridDim.x : gridDim.x / CG;   // SPLIT: one unit
@@ -182,9 +185,12 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
             for (uint32_t kb = 0; kb < KB; kb++, st.next(a.stages)) {
                 if (!(ok = i8_wait<CG>(empty_bar(st.s), st.phase ^ 1u, abort_flag, a.err, 1))) break;
                 if (elect_one()) {
-                    if (rank == 0) mbar_expect_tx(full_bar(st.s), CG * A_TILE);
-                    const uint32_t dst = smem_base + st.s * stage_bytes; const int x = (int)((kb0 + kb) * 128u);
-                    if (CG == 1 && a.once) tma_load_2d_hint(dst, &tm_w, full_bar(st.s), x, wy, policy); else i8_load<CG>(dst, &tm_w, filled_bar(st.s), x, wy);
+                    if (rank == 0) mbar_expect_tx(full_bar(st.s), CG * KPS * A_TILE);
+#pragma unroll
+                    for (uint32_t h = 0; h < KPS; h++) {   // columns past the end are filled with zeros
+                        const uint32_t dst = smem_base + st.s * stage_bytes + h * A_TILE; const int x = (int)(((kb0 + kb) * KPS + h) * 128u);
+                        if (CG == 1 && a.once) tma_load_2d_hint(dst, &tm_w, full_bar(st.s), x, wy, policy); else i8_load<CG>(dst, &tm_w, filled_bar(st.s), x, wy);
+                    }
                 }
                 __syncwarp();
             }
@@ -205,9 +211,12 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
                 if (!(ok = i8_wait<CG>(full_bar(st.s), st.phase, abort_flag, a.err, 3))) break;
                 tc_fence_after();
                 if (elect_one()) {
-                    const uint64_t dw = umma_desc(smem_base + st.s * stage_bytes), dx = umma_desc(smem_base + st.s * stage_bytes + A_TILE);
 #pragma unroll
-                    for (uint32_t ks = 0; ks < 4; ks++) i8_mma<CG>(d, dw + 2u * ks, dx + 2u * ks, idesc, kb | ks);   // 32 columns each
+                    for (uint32_t h = 0; h < KPS; h++) {
+                        const uint64_t dw = umma_desc(smem_base + st.s * stage_bytes + h * A_TILE), dx = umma_desc(smem_base + st.s * stage_bytes + KPS * A_TILE + h * x_tile);
+#pragma unroll
+                        for (uint32_t ks = 0; ks < 4; ks++) i8_mma<CG>(d, dw + 2u * ks, dx + 2u * ks, idesc, kb | h | ks);   // 32 columns each
+                    }
                     i8_commit<CG>(empty_bar(st.s));
                 }
                 __syncwarp();
@@ -226,8 +235,11 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
                 for (uint32_t kb = 0; kb < KB; kb++, st.next(a.stages)) {
                     if (!(ok = i8_wait<CG>(empty_bar(st.s), st.phase ^ 1u, abort_flag, a.err, 6))) break;
                     if (elect_one()) {
-                        if (rank == 0) mbar_expect_tx(full_bar(st.s), CG * boxes * a.box * 128u);
-                        for (uint32_t i = 0; i < boxes; i++) i8_load<CG>(smem_base + st.s * stage_bytes + A_TILE + i * a.box * 128u, &tm_x, filled_bar(st.s), (int)((kb0 + kb) * 128u), y + (int)(i * a.box));
+                        if (rank == 0) mbar_expect_tx(full_bar(st.s), CG * KPS * boxes * a.box * 128u);
+#pragma unroll
+                        for (uint32_t h = 0; h < KPS; h++)
+                            for (uint32_t i = 0; i < boxes; i++)
+                                i8_load<CG>(smem_base + st.s * stage_bytes + KPS * A_TILE + h * x_tile + i * a.box * 128u, &tm_x, filled_bar(st.s), (int)(((kb0 + kb) * KPS + h) * 128u), y + (int)(i * a.box));
                     }
                     __syncwarp();
                 }
@@ -328,7 +340,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
         // ---------------------------------------------------------------- row copies: each of `team` warps fills every team-th stage
         // No more warps than stages: a warp that waits for a place in the ring has then had one since the place's last turn began, and the barrier's parity tells the turns apart.
         constexpr uint32_t team = 4;
-        static_assert((I8_SMEM - 1024 - I8_EPI * I8_OUT) / (A_TILE + I8_N_MAX * 128) >= team, "a ring of as many stages as copying warps");
+        static_assert(I8_ROOM / (A_TILE + I8_N_MAX * 128) >= team, "a ring of as many stages as copying warps");
         // A stage is passed on once its copies have landed and are fenced for the tensor cores' reads; a.lag = 1: when the warp's next stage has been requested,
         // which takes more than 2 * team stages in the ring (every wait for a free stage is then for one that has been passed on).
         if constexpr (GATHER) {
@@ -360,11 +372,14 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
                 if (u + step < total) rows = fetch(u + step);   // a unit ahead: the map's values are there when they are needed
                 for (uint32_t kb = turn; kb < KB; kb += team) {
                     if (!(ok = __all_sync(0xffffffffu, i8_wait<CG>(empty_bar(st.s), st.phase ^ 1u, abort_flag, a.err, 7)))) break;
-                    const uint32_t dst = smem_base + st.s * stage_bytes + A_TILE + r0 * 128u, at = kb * 128u + c * 16u, take = at < a.k ? 16u : 0u;
-                    const int8_t *from = a.x + (take ? at : 0u);
                     // the 128-byte swizzle: 16-byte column c of row r lies at column c ^ (r % 8)
+#pragma unroll
+                    for (uint32_t h = 0; h < KPS; h++) {
+                        const uint32_t dst = smem_base + st.s * stage_bytes + KPS * A_TILE + h * x_tile, at = (kb * KPS + h) * 128u + c * 16u, take = at < a.k ? 16u : 0u;
+                        const int8_t *from = a.x + (take ? at : 0u);
 #pragma unroll 8
-                    for (uint32_t r = r0; r < have; r += 4u) copy16(dst + (r - r0) * 128u + ((c ^ (r & 7u)) << 4), from + (size_t)src[r] * a.x_stride, take);
+                        for (uint32_t r = r0; r < have; r += 4u) copy16(dst + r * 128u + ((c ^ (r & 7u)) << 4), from + (size_t)src[r] * a.x_stride, take);
+                    }
                     asm volatile("cp.async.commit_group;" ::: "memory");
                     if (a.lag == 0u) { copies_wait<0>(); pass_on(); }
                     else if (behind) { copies_wait<1>(); pass_on(); }
@@ -424,9 +439,9 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
     }
 }
 
-template <int CG, bool GATHER, bool SPLIT>
+template <int CG, bool GATHER, bool SPLIT, int KPS>
 static cudaError_t i8_mma_start(const CUtensorMap &w, const CUtensorMap &x, const I8MmaArgs &a, uint32_t grid, cudaStream_t s) {
-    auto kernel = i8_mma_kernel<CG, GATHER, SPLIT>;
+    auto kernel = i8_mma_kernel<CG, GATHER, SPLIT, KPS>;
     // set on every call: it belongs to the device's context and costs well under a launch
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)I8_SMEM);
     if (e != cudaSuccess) return e;
@@ -437,8 +452,15 @@ static cudaError_t i8_mma_start(const CUtensorMap &w, const CUtensorMap &x, cons
     return cudaLaunchKernelEx(&cfg, kernel, w, x, a);
 }
 
+// 128 or 256 columns in a stage. Two blocks halve the barriers' turns, which cost 0.04 us each; they want an even number of blocks in every part, and three stages, five where warps
+// copy the rows (four of 64 rows: 66.1 us instead of 64.8). 300 x 4096 x 2048: 7.4 -> 6.7 us, 64 x 4096 x 4096: 7.8 -> 7.65, 64 tokens through 128 experts: gate|up 50.8 -> 50.0 and
+// down 27.0 -> 26.0. Pairs take 0.25 us for a block's products alone: 4096 x 4096 x 4096 48.4 -> 49.3, so they stay with one.
+static bool i8_two_blocks(uint32_t cg, uint32_t rows, uint32_t kb, uint32_t split, bool gather) {
+    return cg == 1u && kb % (2u * (split > 1u ? split : 1u)) == 0u && I8_ROOM / (2u * (A_TILE + rows * 128u)) >= (gather ? 5u : 3u);
+}
+
 // Form and tile of a dense product: the least estimate, in us, over tile counts that divide the rows evenly. Measured with r rows in a tile, on L2-resident operands:
-// 128 columns take 0.22 + 0.00042 r and at least 0.26 with one CTA, 0.15 + 0.0004 r and at least 0.19 with a pair, whose start costs 1.4 more; a unit's drain keeps a later one
+// 128 columns take 0.22 + 0.00042 r and at least 0.26 with one CTA (0.04 less where a stage holds two blocks), 0.15 + 0.0004 r and at least 0.19 with a pair, whose start costs 1.4 more; a unit's drain keeps a later one
 // waiting from 0.5 + 0.013 r on and costs 0.2 + 0.008 r where none follows; a split costs 1.4 + 0.4 log2(parts) + 0.014 r. 64 x 4096 x 4096: 10.3 us in one part, 8.7 in two, 7.5 in
 // four; 30 x 512 x 4096: 10.0, 8.1, 6.5, 5.8 in eight; 300 x 4096 x 2048: 7.6 with tiles of 80, 8.2 of 160, 11.0 of 64 (two rounds), 8.8 in pairs.
 struct I8Form { uint32_t cg, tiles, split; };
@@ -449,7 +471,10 @@ static I8Form i8_dense_form(uint32_t m, uint32_t n, uint32_t k, uint32_t sms) {
         const uint32_t blocks = (n + 128u * g - 1u) / (128u * g), steps = (m + 16u * g - 1u) / (16u * g), most = I8_N_MAX / (16u * g), least = (steps + most - 1u) / most, workers = sms / g;
         for (uint32_t t = least; t < least + 24u && t <= steps; t++) {
             const float r = (float)((steps + t - 1u) / t * (16u * g)), mean = fmaxf((float)m / t, 16.0f);   // rows of the longest tile, of all
-            const float each = g == 1u ? fmaxf(0.26f, 0.22f + 0.00042f * mean) : fmaxf(0.19f, 0.15f + 0.0004f * mean);
+            auto block = [&](uint32_t split) {
+                return g == 1u ? fmaxf(0.26f, 0.22f + 0.00042f * mean) - (i8_two_blocks(g, (uint32_t)r, kb, split, false) ? 0.04f : 0.0f) : fmaxf(0.19f, 0.15f + 0.0004f * mean);
+            };
+            const float each = block(1u);
             const uint64_t units = (uint64_t)t * blocks;
             const float cost = (float)((units + workers - 1u) / workers) * fmaxf(kb * each, 0.5f + 0.013f * mean) + 0.2f + 0.008f * r + (g == 2u ? 1.4f : 0.0f);
             if (cost < best) { best = cost; f = {g, t, 1u}; }
@@ -457,7 +482,7 @@ static I8Form i8_dense_form(uint32_t m, uint32_t n, uint32_t k, uint32_t sms) {
             uint32_t room = sms;   // clusters of 4 and 8 do not fill the SMs of every group that a cluster has to lie in: 16 of 8 took two rounds
             for (uint32_t s = 2, lg = 1; s <= 8u && s <= kb; s *= 2u, lg++, room -= sms / 8u) {
                 if (units * s > room) break;
-                const float split = (float)((kb + s - 1u) / s) * each + 1.4f + 0.4f * lg + 0.014f * r;
+                const float split = (float)((kb + s - 1u) / s) * block(s) + 1.4f + 0.4f * lg + 0.014f * r;
                 if (split < best) { best = split; f = {1u, t, s}; }
             }
         }
@@ -487,17 +512,21 @@ cudaError_t launch_i8_mma(const OmegaGpuI8Tensor *t, const I8Launch &l, cudaStre
     const uint32_t per_cta = a.n_cap / cg;
     a.box = !l.tiles ? per_cta : per_cta % 64u == 0 ? 64u : per_cta % 32u == 0 ? 32u : 16u;
     a.packed = l.y16 && !l.y32 && l.n % 8u == 0;
-    a.stages = (uint32_t)((I8_SMEM - 1024 - I8_EPI * I8_OUT) / (A_TILE + per_cta * 128u)); if (a.stages > I8_STAGES) a.stages = I8_STAGES;
+    const bool two = i8_two_blocks(cg, per_cta, (t->k + 127u) / 128u, a.split, l.xmap != nullptr);
+    a.stages = I8_ROOM / ((A_TILE + per_cta * 128u) * (two ? 2u : 1u)); if (a.stages > I8_STAGES) a.stages = I8_STAGES;
     a.lag = a.stages > 7u;
     a.tmem_cols = 32; while (a.tmem_cols < 2u * a.n_cap) a.tmem_cols *= 2;
     CUtensorMap w, x;
     if (!make_tmap_u8(&w, t->w, t->n, t->k, 128) || !make_tmap_u8(&x, l.x, l.x_rows, t->k, a.box, l.x_stride)) return cudaErrorInvalidValue;
     const uint64_t units = (uint64_t)a.tiles_most * a.cblocks;
     if (units > 0x7fffffffull) return cudaErrorInvalidValue;
-    if (a.split > 1u) return i8_mma_start<1, false, true>(w, x, a, (uint32_t)units * a.split, s);
-    uint32_t grid = (uint32_t)(units * cg < sms ? units * cg : sms); grid -= grid % cg;
-    if (cg == 2u) return i8_mma_start<2, false, false>(w, x, a, grid, s);
-    return l.xmap ? i8_mma_start<1, true, false>(w, x, a, grid, s) : i8_mma_start<1, false, false>(w, x, a, grid, s);
+    uint32_t grid = a.split > 1u ? (uint32_t)units * a.split : (uint32_t)(units * cg < sms ? units * cg : sms); grid -= grid % cg;
+    if (cg == 2u) return i8_mma_start<2, false, false, 1>(w, x, a, grid, s);
+#define I8_START(GATHER, SPLIT) return two ? i8_mma_start<1, GATHER, SPLIT, 2>(w, x, a, grid, s) : i8_mma_start<1, GATHER, SPLIT, 1>(w, x, a, grid, s)
+    if (a.split > 1u) I8_START(false, true);
+    if (l.xmap) I8_START(true, false);
+    I8_START(false, false);
+#undef I8_START
 }
 
 }  // namespace b200

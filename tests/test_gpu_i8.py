@@ -290,6 +290,19 @@ def test_large_products(m, n, k):
     api.lib.omega_gpu_i8_free(t)
 
 
+@pytest.mark.parametrize("m,n,k", [(300, 1024, 1936), (130, 6144, 1008), (64, 1030, 4096), (40, 500, 3968), (33, 264, 2000), (200, 4100, 2304), (600, 2048, 512)])
+def test_products_of_two_blocks_a_stage(m, n, k):
+    """256 columns in a stage, in one part and in several, with ragged last blocks, and an odd number of blocks next to them"""
+    test_large_products(m, n, k)
+
+
+@pytest.mark.parametrize("tile_rows", [5, 16, 32, 48])
+@pytest.mark.parametrize("n,k", [(640, 1008), (520, 1152), (300, 2048)])
+def test_grouped_product_around_the_ring(tile_rows, n, k):
+    """more units than workers, so that the stages' turns run on from one unit into the next"""
+    test_grouped_product(tile_rows, 160, 3, 40, n, k, 0)
+
+
 @pytest.mark.parametrize("m", [1, 12, 17, 40, 90, 200, 300, 777])
 @pytest.mark.parametrize("n,k", [(8, 64), (136, 528), (100, 256), (264, 4112), (1032, 2048)])
 def test_bf16_rows_are_the_f32_ones_rounded(m, n, k):
