@@ -26,6 +26,7 @@ struct RouteArgs {
 };
 
 constexpr uint32_t ROUTE_WARPS = 4, ROUTE_MOST_TOKENS = 1u << 30;
+constexpr float TINY = 1e-36f;           // below it f32 scores may have lost their relative error bound: subnormal numbers, and quotients of 2^126 and more
 constexpr uint32_t KEY_NAN = 1;          // below the key of -infinity; 0 = not to be picked
 __device__ __forceinline__ uint32_t order_key(float v) {   // larger float, larger key; NaN lowest
     const uint32_t b = __float_as_uint(v);                 // never -0: scores are not, and a sum is only where both parts are
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, VPL <= 8 ? 8 : 2) score_rout
                 if (m == best) m = 0;
             }
             const float edge = key_value(least);
-            if (least > KEY_NAN && fabsf(edge) <= 3.0e38f) least = order_key(edge - (a.bias ? 4e-6f * most + 5e-7f * fabsf(edge) : 1e-4f * edge));
+            if (least > KEY_NAN && fabsf(edge) <= 3.0e38f) least = order_key(a.bias ? edge - (4e-6f * most + 5e-7f * fabsf(edge)) : edge < TINY ? 0.0f : edge - 1e-4f * edge);
             uint32_t n = 0;
 #pragma unroll
             for (int i = 0; i < VPL; i++) {
@@ -205,10 +206,11 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, VPL <= 8 ? 8 : 2) score_rout
             __syncwarp();
             if (n <= 32u) {
                 uint64_t mine = 0;
+                float my_l = -INFINITY;
                 if (lane < n) {
                     const uint32_t e = (uint32_t)s_cand[warp][lane];
                     const float v = a.bf16 ? __uint_as_float((uint32_t) reinterpret_cast<const uint16_t *>(row)[e] << 16) : reinterpret_cast<const float *>(row)[e];
-                    my_id = e;
+                    my_id = e; my_l = v;
                     my_s = a.sigmoid ? (float)score(v) : (float)(score(v) / (sum > 0.0 ? sum : 1.0));
                     mine = ((uint64_t)order_key(v != v ? v : a.bias ? my_s + a.bias[e] : my_s) << 32) | ~e;   // ~e: the lowest index of equals first
                 }
@@ -223,6 +225,8 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, VPL <= 8 ? 8 : 2) score_rout
                     __syncwarp();
                     if (lane < n) s_cand[warp][place] = mine;
                     __syncwarp();
+                    // (rounded to a subnormal number, 4e-7 of a score may be a whole unit of it)
+                    if (!a.bias && lane < n && place < a.topk && (uint32_t)(mine >> 32) > KEY_NAN) near |= my_s < TINY && my_l != -INFINITY;
                     const uint64_t next = place < a.topk && place + 1u < n ? s_cand[warp][place + 1u] : 0;
                     if ((uint32_t)(next >> 32) > KEY_NAN) {
                         const float v = key_value((uint32_t)(mine >> 32)), w = key_value((uint32_t)(next >> 32));

@@ -100,6 +100,34 @@ def test_route_scores_a_unit_in_the_last_place_apart(sigmoid, biased, E, groups,
             check_route(l, bias, E, topk, sigmoid, groups, kept, 2 if groups > 1 else 1)
 
 
+@pytest.mark.parametrize("sigmoid", [True, False])
+@pytest.mark.parametrize("E,groups,kept", [(24, 1, 0), (64, 1, 0), (256, 8, 4), (600, 1, 0)])
+def test_route_picks_among_scores_below_the_normal_numbers(sigmoid, E, groups, kept):
+    """no bias, and picks whose scores are a few units of the smallest float: many are equal once rounded, and the lowest index has to come first"""
+    rng = np.random.default_rng(E)
+    l = np.empty((60, E), np.float32)
+    for t in range(60):
+        l[t] = rng.uniform(-103.5, -86.0, E) if t % 2 else -95.0 + rng.uniform(0, 2e-3, E)
+        if not sigmoid:
+            l[t] += 90.0
+            l[t, :: max(1, E // 3)] = 90.0                                   # three or four take it all
+    for topk in (2, 8, 20):
+        if topk <= (kept or groups) * (E // groups):
+            check_route(l, None, E, topk, sigmoid, groups, kept, 2 if groups > 1 else 1)
+
+
+def test_route_softmax_scores_that_round_to_the_same_tiny_float():
+    """seven clear picks, and an eighth among two dozen scores of 48 to 51 units of the smallest float: equal once rounded, though a rounded exponential times a rounded factor is not"""
+    rng = np.random.default_rng(8)
+    l = np.full((400, 128), -np.inf, np.float32)
+    for t in range(400):
+        at = rng.permutation(np.arange(0, 128, 4))
+        l[t, at[:7]] = (90.0, 89.9, 89.7, 60.0, 50.0, 40.0, 30.0)
+        total = np.exp(l[t, at[:7]].astype(np.float64) - 90.0).sum()
+        l[t, at[7:]] = 90.0 + np.log(total * rng.uniform(48.3, 50.7, 25) * 2.0 ** -149)
+    check_route(l, None, 128, 8, False)
+
+
 def test_route_strided_rows_on_another_stream():
     import torch
     rng = np.random.default_rng(5)
