@@ -85,7 +85,8 @@ __global__ void __launch_bounds__(W * 32) norm_q8_kernel(uint32_t hidden, float 
 #pragma unroll
     for (int i = 0; i < W; i++) { a += r_sq[i]; top = max(top, r_top[i]); }
     const double rms = sqrt(a / (double)hidden + (double)eps);
-    const float pre = rms > 1.2676506002282294e30 /* 2^100 */ ? 5.421010862427522e-20f /* 2^-64 */ : 1.0f;   // keeps the factor of huge rows out of the subnormal numbers
+    // keeps the factor of huge rows out of the subnormal numbers and that of tiny ones (no eps) out of the infinite ones
+    const float pre = rms > 1.2676506002282294e30 /* 2^100 */ ? 5.421010862427522e-20f /* 2^-64 */ : rms < 7.888609052210118e-31 /* 2^-100 */ ? 1.8446744073709552e19f /* 2^64 */ : 1.0f;
     const float r = (float)(1.0 / (rms * (double)pre));
     // a row that is not finite has a NaN or an infinity among the h * w (0 * infinity is NaN)
     const uint32_t y_top = top < Q8_INF ? abs_bits(__uint_as_float(top) * pre * r) : Q8_INF;

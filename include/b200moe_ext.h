@@ -301,7 +301,8 @@ int omega_gpu_moe_route(const OmegaGpuMoeRouteConfig *cfg, uint32_t tokens, cons
  * addresses are 16-byte aligned (f32 scales 4). No output may overlap an input, except h_va = h_in_va. */
 /* h = (x16 ? bf16 -> f32(x16) : h_in) + (m ? m : 0); y = h / sqrt(mean(h^2) + eps) * norm_w, quantised. x16_va bf16 or h_in_va f32 [tokens][hidden] (one of them);
  * m_va f32 or (m_bf16) bf16, optional; h_va f32, optional output; norm_w_va f32 [hidden], 0 = ones; xn_bf16_va optional output bf16(y), the rows that a router
- * reads. Beside omega_gpu_residual_norm_w_async, which leaves bf16 rows. A row counts as non-finite when h * norm_w leaves the f32 range. */
+ * reads. Beside omega_gpu_residual_norm_w_async, which leaves bf16 rows. A row counts as non-finite when h * norm_w leaves the f32 range, and where
+ * h * norm_w is below 2^-126 (eps 0 and a tiny row) it is rounded as f32 rounds it. */
 int omega_gpu_residual_norm_q8_async(uint32_t tokens, uint32_t hidden, float eps, uint64_t x16_va, uint64_t m_va, int m_bf16, uint64_t h_in_va, uint64_t h_va,
                                      uint64_t norm_w_va, uint64_t xn_bf16_va, uint64_t q_va, uint64_t s_va, void *stream);
 /* rows as they are: x_va bf16 (x_bf16 != 0) or f32, x_stride_bytes apart (0 = dense; a multiple of 16) */

@@ -203,6 +203,15 @@ def test_norm_rows_at_the_edges(H):
     assert np.isnan(s0[0])                                                   # 0 / 0
 
 
+@pytest.mark.parametrize("H", [16, 2048])
+def test_norm_of_tiny_rows_without_eps(H):
+    """mean squares whose root's reciprocal leaves the f32 range"""
+    rng = np.random.default_rng(H)
+    x = rng.normal(0, 1, (5, H)).astype(np.float32) * np.float32([1e-20, 1e-30, 1e-37, 1e-39, 1e-42])[:, None]
+    rc, _, q, s = api.residual_norm_q8_f32(x, None, None, eps=0.0); ok(rc)
+    check_rows(q, s, ref.norm(x.astype(np.float64), None, 0.0), 4 * EPS24)
+
+
 # the fast exponential is off by (2 + 1.173 |g|) 2^-23, its quotient by 2 more units, the product by one rounding
 GATE_REL = lambda g: ((2 + 1.173 * g) + 2) * 2.0 ** -23 + EPS24              # noqa: E731
 
