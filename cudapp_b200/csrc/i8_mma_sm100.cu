@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
     if (!a.early || warp != 0) griddep_chain();   // early weights are requested while the kernels ahead still run
     const uint32_t total = a.early ? s_total : units();
     const uint32_t first = SPLIT ? blockIdx.x / a.split : blockIdx.x / CG, step = SPLIT ? gridDim.x : gridDim.x / CG;   // SPLIT: one unit
-    auto tile_rows = [](uint32_t cnt) { return (cnt + 16u * CG - 1u) / (16u * CG) * 16u; };   // rows of a tile that this CTA holds
+    auto tile_rows = [](uint32_t cnt) { return cnt ? (cnt + 16u * CG - 1u) / (16u * CG) * 16u : 16u; };   // rows of a tile that this CTA holds; a product has 16 at least, though a plan's tile may have none
     auto filled_bar = [&](uint32_t s) { return CG == 2 ? in_first_cta(full_bar(s)) : full_bar(s); };
 
     if (warp == 0) {
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
             const uint32_t me = warp - (4 + I8_EPI), c = lane & 7u, r0 = lane >> 3;
             uint32_t *src = s_src[me];
             I8Stage st, done; bool ok = true, behind = false;
-            uint32_t ahead[I8_N_MAX / 32], turn = 0;   // turn: stages until this warp's next
+            uint32_t ahead[I8_N_MAX / 32] = {}, turn = 0;   // turn: stages until this warp's next
             for (uint32_t i = 0; i < me; i++) st.next(a.stages);
             done = st; turn = me;
             auto fetch = [&](uint32_t u) {

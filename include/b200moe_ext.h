@@ -326,7 +326,7 @@ int omega_gpu_i8_gemm_async(const OmegaGpuI8Tensor *t, uint32_t m, uint64_t x_va
 /* host buffers, dense */
 int omega_gpu_i8_gemm(const OmegaGpuI8Tensor *t, uint32_t m, const int8_t *x, const float *x_scale, uint16_t *y_bf16, float *y_f32);
 /* Grouped by expert: the tensor was uploaded as experts x (n / experts) rows. The rows to multiply are described by a routing plan (omega_gpu_moe_plan_async) made
- * with tile_rows from 1 to 256: tiles u32 x4 {expert, first sorted row, rows <= tile_rows, -}, header[2] = number of tiles, at most max_tiles. Row i of a tile is
+ * with tile_rows from 1 to 256: tiles u32 x4 {expert, first sorted row, rows <= tile_rows (0: nothing to do), -}, header[2] = number of tiles, at most max_tiles. Row i of a tile is
  * x[xmap[first + i]] with that row's scale (xmap_va 0: x[first + i]); x holds x_rows dense rows. Its result row (n / experts wide) is y[ymap[first + i]]
  * (ymap_va 0: y[first + i]). One launch, nothing allocated. */
 int omega_gpu_i8_gemm_grouped_async(const OmegaGpuI8Tensor *t, uint32_t experts, uint32_t tile_rows, uint32_t max_tiles, uint64_t tiles_va, uint64_t header_va,

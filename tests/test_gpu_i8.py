@@ -426,6 +426,35 @@ def test_grouped_product(tile_rows, T, S, E, n, k, skew):
     api.lib.omega_gpu_i8_free(t)
 
 
+@pytest.mark.parametrize("tile_rows", [16, 48, 160])
+@pytest.mark.parametrize("gathered", [True, False])
+def test_grouped_product_of_a_plan_of_ones_own(tile_rows, gathered):
+    """tiles in any order, experts twice, tiles without rows, at the first place and the last one too"""
+    import torch
+    rng = np.random.default_rng(tile_rows)
+    E, n, k, R = 5, 264, 640, 400
+    counts = [0, tile_rows, 3, 0, 0, 17 % tile_rows, tile_rows - 1, 1, 0]
+    experts = [2, 4, 0, 1, 4, 4, 3, 0, 3]
+    rows = np.cumsum([0] + counts[:-1])
+    tiles = np.zeros((len(counts) + 3, 4), np.uint32)
+    tiles[:len(counts), 0], tiles[:len(counts), 1], tiles[:len(counts), 2] = experts, rows, counts
+    total = int(sum(counts)); assert total <= R
+    x, xs, w, ws = codes(rng, R, k), scales(rng, R), codes(rng, E * n, k), scales(rng, E * n)
+    xmap, ymap = rng.integers(0, R, total).astype(np.uint32), rng.permutation(R)[:total].astype(np.uint32)
+    rc, t = api.i8_upload(w, ws); ok(rc)
+    y, dt, dh = torch.full((R, n), 3.0, device="cuda"), dev(tiles), dev(np.array([0, 0, len(counts), 0], np.uint32))
+    dx, dxs, dxm, dym = dev(x), dev(xs), dev(xmap), dev(ymap)
+    ok(api.lib.omega_gpu_i8_gemm_grouped_async(t, E, tile_rows, len(tiles), dt.data_ptr(), dh.data_ptr(), dxm.data_ptr() if gathered else 0, dym.data_ptr(), dx.data_ptr(), R, dxs.data_ptr(), 0, y.data_ptr(), here()))
+    assert api.lib.omega_gpu_i8_status(t, here()) == 0
+    want = np.full((R, n), 3.0)
+    for e, r0, c in zip(experts, rows, counts):
+        for r in range(r0, r0 + c):
+            src = xmap[r] if gathered else r
+            want[ymap[r]] = ref.gemm(x[src:src + 1], xs[src:src + 1], w[e * n:(e + 1) * n], ws[e * n:(e + 1) * n])[0]
+    assert np.all(np.abs(y.cpu().numpy() - want) <= 3 * EPS24 * np.abs(want))
+    api.lib.omega_gpu_i8_free(t)
+
+
 def test_grouped_product_after_a_refused_plan_does_nothing():
     import torch
     rng = np.random.default_rng(1)
