@@ -175,14 +175,18 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
     auto tile_rows = [](uint32_t cnt) { return cnt ? (cnt + 16u * CG - 1u) / (16u * CG) * 16u : 16u; };   // rows of a tile that this CTA holds; a product has 16 at least, though a plan's tile may have none
     auto filled_bar = [&](uint32_t s) { return CG == 2 ? in_first_cta(full_bar(s)) : full_bar(s); };
 
+    // Early weights' warp learns here that the kernels ahead are done, from warp 3, which has waited for them: a wait of its own so late takes 2 us (64 x 4096 x 4096: 7.7 -> 9.7)
+    auto ahead_done = []() { asm volatile("barrier.sync 1, 64;" ::: "memory"); };
+    if (a.early && warp == 3) asm volatile("barrier.arrive 1, 64;" ::: "memory");
     if (warp == 0) {
         // ---------------------------------------------------------------- weights
         const uint64_t policy = l2_policy_evict_first();
-        I8Stage st; bool ok = true;
+        I8Stage st; bool ok = true, waited = !a.early;
         for (uint32_t u = first; u < total && ok; u += step) {
             const I8Unit t = i8_unit<CG>(a, u);
             const int wy = (int)(t.expert * a.n + t.c0 + rank * 128u);
             for (uint32_t kb = 0; kb < KB; kb++, st.next(a.stages)) {
+                if (!waited && st.phase) { ahead_done(); waited = true; }   // the ring is full: until the kernels ahead are done nothing empties it, and they may outlast a bounded wait
                 if (!(ok = i8_wait<CG>(empty_bar(st.s), st.phase ^ 1u, abort_flag, a.err, 1))) break;
                 if (elect_one()) {
                     if (rank == 0) mbar_expect_tx(full_bar(st.s), CG * KPS * A_TILE);
@@ -195,6 +199,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
                 __syncwarp();
             }
         }
+        if (!waited) ahead_done();
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer
         // the whole warp walks through the loop, one lane issues: addresses and descriptors then stay in uniform registers
@@ -394,7 +399,6 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
     }
     if constexpr (SPLIT) {
         // ---------------------------------------------------------------- the parts' sums: every split-th row, two rows of 128 channels at a time per warp
-        if (warp == 0) griddep_wait();   // the one that has not: it reads scales and writes results now
         __syncwarp();
         cluster_sync();
         const uint32_t warps = blockDim.x / 32u, c = (lane & 15u) * 4u;
