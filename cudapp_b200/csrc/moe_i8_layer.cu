@@ -70,16 +70,16 @@ struct OmegaGpuMoeI8Layer {
 };
 
 namespace b200 {
-// Rows per tile: an expert's average and half of it again, so that most experts are one tile, which reads their weights once, and a tile leaves the pipeline its stages; the
-// longest where that is more than 96. Measured, 128 experts of 2048 x 768 with an uneven load, us: 512 tokens 147 / 134 / 140 / 150 with 32 / 64 / 96 / 128 rows; 1024 tokens
-// 163 / 160 / 171 / 167 with 64 / 96 / 128 / 256; 2048 tokens 222 / 221 / 211 / 207 with 96 / 128 / 192 / 256.
+// Rows per tile: room for an expert's average and half of it again while that is 32 or 64, so that most experts are one tile, which reads their weights once, and a tile leaves the
+// pipeline its stages; above that the longest, in pairs of CTAs. Measured, 128 experts of 2048 x 768 with an uneven load, us with 64 / 96 / 128 / 256 rows: 512 tokens (32 an
+// expert) 127 / 138 / 140 / 142, 768 tokens 143 / 150 / 150 / 151, 1024 tokens 163 / 161 / 158 / 158, 1500 tokens 195 / 196 / 179 / 176, 4096 tokens 436 / 412 / 320 / 290.
 static uint32_t i8_tile_rows(uint32_t picks, uint32_t experts) {
-    const uint32_t rows = (3u * (picks / experts) / 2u + 31u) / 32u * 32u;
-    return rows < 32u ? 32u : rows > 96u ? 256u : rows;
+    const uint32_t average = picks / experts;
+    return average <= 21u ? 32u : average <= 56u ? 64u : 256u;
 }
 // Rows are copied into sorted order first where tiles are long: the product then fetches a tile's rows by TMA, which costs less than their copies through the
-// map once a row is used by several channel blocks of a long tile. Measured: 512 tokens (32 rows an expert) 129.6 us unsorted, 133.7 sorted, 1024 tokens 169.8 and 171.2;
-// gate|up alone of 4096 tokens 122 us and 14 for the copies against 216.
+// map once a row is used by several channel blocks of a long tile. Measured: 512 tokens (32 rows an expert) 129.6 us unsorted, 133.7 sorted; gate|up alone of 4096 tokens
+// 114 us and 14 for the copies against 199.
 static bool i8_sorted(uint32_t picks, uint32_t experts) { return i8_tile_rows(picks, experts) == 256u; }
 static uint32_t i8_max_tiles(uint32_t picks, uint32_t experts, uint32_t tile_rows) { return picks / tile_rows + (experts < picks ? experts : picks); }
 
