@@ -48,20 +48,6 @@ __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("m
 __device__ __forceinline__ uint32_t in_first_cta(uint32_t addr) { uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr)); return r; }
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
-// the bounded wait of mma_common.cuh, seeing what the other CTA of a pair released
-template <int CG> __device__ __forceinline__ bool i8_wait(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag, uint32_t *err, uint32_t code) {
-    if constexpr (CG == 1) return mbar_wait(bar, parity, abort_flag, err, code);
-    else {
-        for (uint32_t i = 0; i < SPIN_LIMIT; i++) {
-            uint32_t ok;
-            asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-            if (ok) return true;
-            if ((i & 255u) == 255u && *abort_flag) return false;
-        }
-        *abort_flag = 1; atomicCAS(err, 0u, code);
-        return false;
-    }
-}
 template <int CG> __device__ __forceinline__ void i8_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
     if constexpr (CG == 1) tma_load_2d(dst, map, bar, x, y);
     else asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
@@ -187,7 +173,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
             const int wy = (int)(t.expert * a.n + t.c0 + rank * 128u);
             for (uint32_t kb = 0; kb < KB; kb++, st.next(a.stages)) {
                 if (!waited && st.phase) { ahead_done(); waited = true; }   // the ring is full: until the kernels ahead are done nothing empties it, and they may outlast a bounded wait
-                if (!(ok = i8_wait<CG>(empty_bar(st.s), st.phase ^ 1u, abort_flag, a.err, 1))) break;
+                if (!(ok = mbar_wait(empty_bar(st.s), st.phase ^ 1u, abort_flag, a.err, 1))) break;
                 if (elect_one()) {
                     if (rank == 0) mbar_expect_tx(full_bar(st.s), CG * KPS * A_TILE);
 #pragma unroll
@@ -210,10 +196,10 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
             // D s32, A = B = signed 8-bit, both K-major, M 128 CG, N cols
             const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((cols >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
             const uint32_t d = tmem + buf * a.n_cap;
-            if (!(ok = i8_wait<CG>(accempty_bar(buf), acc.phase ^ 1u, abort_flag, a.err, 2))) break;
+            if (!(ok = mbar_wait(accempty_bar(buf), acc.phase ^ 1u, abort_flag, a.err, 2))) break;
             tc_fence_after();
             for (uint32_t kb = 0; kb < KB; kb++, st.next(a.stages)) {
-                if (!(ok = i8_wait<CG>(full_bar(st.s), st.phase, abort_flag, a.err, 3))) break;
+                if (!(ok = mbar_wait(full_bar(st.s), st.phase, abort_flag, a.err, 3))) break;
                 tc_fence_after();
                 if (elect_one()) {
 #pragma unroll
@@ -238,7 +224,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
                 const uint32_t rows = tile_rows(t.cnt), boxes = (rows + a.box - 1u) / a.box;
                 const int y = (int)(t.row0 + rank * rows);
                 for (uint32_t kb = 0; kb < KB; kb++, st.next(a.stages)) {
-                    if (!(ok = i8_wait<CG>(empty_bar(st.s), st.phase ^ 1u, abort_flag, a.err, 6))) break;
+                    if (!(ok = mbar_wait(empty_bar(st.s), st.phase ^ 1u, abort_flag, a.err, 6))) break;
                     if (elect_one()) {
                         if (rank == 0) mbar_expect_tx(full_bar(st.s), CG * KPS * boxes * a.box * 128u);
 #pragma unroll
@@ -280,7 +266,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
             __syncwarp();
             if (lane == 0) mbar_arrive(all_bar);
             if (!(ok = mbar_wait(all_bar, n & 1u, abort_flag, a.err, 5))) break;
-            if (!(ok = i8_wait<CG>(accfull_bar(buf), acc.phase, abort_flag, a.err, 4))) break;
+            if (!(ok = mbar_wait(accfull_bar(buf), acc.phase, abort_flag, a.err, 4))) break;
             tc_fence_after();
             // The accumulator is handed back as soon as this warp's last load from it has landed (tcgen05.wait::ld), ahead of the results' way out. In a pair the arrival crosses to the
             // other CTA: it orders nothing but those loads, and releasing at cluster scope would wait for the stores before it to be acknowledged (a 4096-token layer's down product
@@ -384,7 +370,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
                 __syncwarp();
                 if (u + step < total) rows = fetch(u + step);   // a unit ahead: the map's values are there when they are needed
                 for (uint32_t kb = turn; kb < KB; kb += team) {
-                    if (!(ok = __all_sync(0xffffffffu, i8_wait<CG>(empty_bar(st.s), st.phase ^ 1u, abort_flag, a.err, 7)))) break;
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(st.s), st.phase ^ 1u, abort_flag, a.err, 7)))) break;
                     // the 128-byte swizzle: 16-byte column c of row r lies at column c ^ (r % 8)
 #pragma unroll
                     for (uint32_t h = 0; h < KPS; h++) {
