@@ -268,15 +268,15 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
             if (!(ok = mbar_wait(all_bar, n & 1u, abort_flag, a.err, 5))) break;
             if (!(ok = mbar_wait(accfull_bar(buf), acc.phase, abort_flag, a.err, 4))) break;
             tc_fence_after();
-            // The accumulator is handed back as soon as this warp's last load from it has landed (tcgen05.wait::ld), ahead of the results' way out. In a pair the arrival crosses to the
-            // other CTA: it orders nothing but those loads, and releasing at cluster scope would wait for the stores before it to be acknowledged (a 4096-token layer's down product
-            // 78 us, 90 with a release after the stores).
+            // A pair's accumulator is handed back as soon as this warp's last load from it has landed (tcgen05.wait::ld), ahead of the results' way out. The arrival crosses to the other
+            // CTA: it orders nothing but those loads, and releasing at cluster scope would wait for the stores before it to be acknowledged (a 4096-token layer's down product 78 us, 90
+            // with a release after the stores). One CTA's is handed back after the stores have been issued: its units are many and short, and 64 tokens take 79 us so, 82 the other way.
             auto hand_back = [&]() {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) { if constexpr (CG == 2) mbar_arrive_cluster_relaxed(in_first_cta(accempty_bar(buf))); else mbar_arrive(accempty_bar(buf)); }
             };
-            if (sub * 16u >= t.cnt) hand_back();   // no rows of this warp
+            if (CG == 2 && sub * 16u >= t.cnt) hand_back();   // no rows of this warp
             const uint32_t taddr = tmem + ((quarter * 32u) << 16) + buf * a.n_cap, ch0 = t.c0 + rank * 128u + quarter * 32u;
             if constexpr (SPLIT) {   // the stages have been read: their memory takes the sums, [row][channel]
                 for (uint32_t c = sub * 16u; c < t.cnt; c += 64u) {
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
                 if (sub * 16u < t.cnt) { TMEM_LD16X256(taddr + sub * 16u, v, 0); TMEM_LD16X256(taddr + (16u << 16) + sub * 16u, v, 8); }
                 for (uint32_t c = sub * 16u; c < t.cnt; c += 64u) {
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (c + 64u >= t.cnt) hand_back();
+                    if (CG == 2 && c + 64u >= t.cnt) hand_back();
                     uint32_t o[8];
                     const float2 x0 = *reinterpret_cast<const float2 *>(&s_xs[p][c + 2u * part]), x1 = *reinterpret_cast<const float2 *>(&s_xs[p][c + 8u + 2u * part]);
 #pragma unroll
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
                     uint32_t v[16];
                     TMEM_LD16(taddr + c, v, 0);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (c + 64u >= t.cnt) hand_back();
+                    if (CG == 2 && c + 64u >= t.cnt) hand_back();
                     if (ch0 + lane < a.n) {
 #pragma unroll
                         for (uint32_t i = 0; i < 16; i++) {
@@ -334,6 +334,7 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
                     __syncwarp();
                 }
             }
+            if (CG == 1) hand_back();
         }
     } else if (GATHER && warp >= 4 + I8_EPI) {
         // ---------------------------------------------------------------- row copies: each of `team` warps fills every team-th stage
