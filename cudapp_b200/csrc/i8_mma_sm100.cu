@@ -499,7 +499,7 @@ cudaError_t launch_i8_mma(const OmegaGpuI8Tensor *t, const I8Launch &l, cudaStre
     uint32_t cg = 1;
     if (l.tiles) {
         a.tiles_most = l.m;
-        cg = !l.xmap && l.tile_rows >= 128u ? 2u : 1u;   // long tiles in pairs: a layer of 4096 tokens 328 us instead of 334 in a run of many
+        cg = !l.xmap && l.tile_rows >= 128u ? 2u : 1u;   // long tiles in pairs: a layer of 4096 tokens 288 us instead of 307, of 1500 tokens 174 instead of 183
         a.n_cap = (l.tile_rows + 16u * cg - 1u) / (16u * cg) * (16u * cg);
     }
     else {
