@@ -357,6 +357,35 @@ def test_bf16_rows_are_the_f32_ones_rounded(m, n, k):
     api.lib.omega_gpu_i8_free(t)
 
 
+def test_offsets_past_32_bits():
+    """results, rows and codes of more than 2^32 elements: first and last rows of each"""
+    import torch
+    g = torch.Generator(device="cuda"); g.manual_seed(2)
+    m, n, k = 66000, 66000, 64
+    x, w = (torch.randint(-128, 128, s, generator=g, dtype=torch.int8, device="cuda") for s in ((m, k), (n, k)))
+    xs, ws = torch.rand(m, generator=g, device="cuda") + 0.5, torch.rand(n, generator=g, device="cuda") + 0.5
+    rc, t = api.i8_upload_dev(n, k, w.data_ptr(), ws.data_ptr()); ok(rc)
+    y = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+    ok(api.lib.omega_gpu_i8_gemm_async(t, m, x.data_ptr(), 0, xs.data_ptr(), y.data_ptr(), 0, here()))
+    assert api.lib.omega_gpu_i8_status(t, here()) == 0
+    for rows in (slice(0, 40), slice(32500, 32540), slice(m - 40, m)):
+        want = (x[rows].double() @ w.double().T) * torch.outer(xs[rows].double(), ws.double())
+        assert bool(((y[rows].double() - want).abs() <= (BF16_HALF * (1 + 2 ** -7) + 4 * EPS24) * want.abs()).all())
+    del y, x, w
+    api.lib.omega_gpu_i8_free(t)
+    T, H = 270000, 16000                                                     # 4.3e9 elements
+    x = torch.empty((T, H), dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    q, s = torch.empty((T, H), dtype=torch.int8, device="cuda"), torch.empty(T, device="cuda")
+    ends = (slice(0, 5), slice(T - 5, T))
+    host = [x[r].double().cpu().numpy() for r in ends]
+    ok(api.lib.omega_gpu_quant_q8_async(T, H, x.data_ptr(), 1, 0, q.data_ptr(), s.data_ptr(), here()))
+    for r, v in zip(ends, host):
+        check_rows(q[r].cpu().numpy(), s[r].cpu().numpy(), v, 0.0)
+    ok(api.lib.omega_gpu_residual_norm_q8_async(T, H, 1e-6, x.data_ptr(), 0, 0, 0, 0, 0, 0, q.data_ptr(), s.data_ptr(), here()))
+    for r, v in zip(ends, host):
+        check_rows(q[r].cpu().numpy(), s[r].cpu().numpy(), ref.norm(v, None, 1e-6), 4 * EPS24)
+
+
 def test_products_on_two_streams_at_once():
     import torch
     rng = np.random.default_rng(11)
