@@ -213,8 +213,10 @@ cudaError_t launch_plan_batch(uint32_t layers, uint32_t tokens, uint32_t slots, 
 // ------------------------------------------------------------------ plan of many picks: three launches, one CTA per 1024 picks in the first and the last
 // The same stable order as plan_kernel (sorted row = rows of lower experts + earlier picks of the same expert), split so that the
 // per-chunk work runs on as many SMs as there are chunks: (1) per-chunk histograms, (2) one CTA turns them into per-chunk
-// offsets and builds the tables, (3) every chunk scatters its picks. scratch: u32 [chunks][experts] + 1 flag word.
-__global__ void __launch_bounds__(1024) plan_hist_kernel(uint32_t R, uint32_t experts, const uint32_t *ids, uint32_t *__restrict__ scratch, uint32_t chunks) {
+// offsets and builds the tables, (3) every chunk scatters its picks. scratch: u32 flag, then [chunks][experts]. The flag has a place that no call's histograms reach: one
+// scratch serves calls of any size, and behind the histograms of a shorter call lie the counts of a longer one.
+constexpr uint32_t PLAN_FLAG = 0, PLAN_HIST = 1;
+__global__ void __launch_bounds__(1024) plan_hist_kernel(uint32_t R, uint32_t experts, const uint32_t *ids, uint32_t *__restrict__ scratch) {
     griddep_chain();
     extern __shared__ uint32_t smem[];
     const uint32_t tid = threadIdx.x;
@@ -223,10 +225,10 @@ __global__ void __launch_bounds__(1024) plan_hist_kernel(uint32_t R, uint32_t ex
     const uint32_t i = blockIdx.x * 1024u + tid;
     if (i < R) {
         const uint32_t e = ids[i];
-        if (e != 0xffffffffu) { if (e >= experts) atomicOr(scratch + (size_t)chunks * experts, 1u); else atomicAdd(&smem[e], 1u); }
+        if (e != 0xffffffffu) { if (e >= experts) atomicOr(scratch + PLAN_FLAG, 1u); else atomicAdd(&smem[e], 1u); }
     }
     __syncthreads();
-    for (uint32_t e = tid; e < experts; e += 1024) scratch[(size_t)blockIdx.x * experts + e] = smem[e];
+    for (uint32_t e = tid; e < experts; e += 1024) scratch[PLAN_HIST + (size_t)blockIdx.x * experts + e] = smem[e];
 }
 // dynamic shared: counts[E] | starts[E] | scan buf[96]
 __global__ void __launch_bounds__(1024) plan_scan_kernel(uint32_t experts, uint32_t tile_rows, uint32_t *__restrict__ scratch, uint32_t chunks, const OmegaGpuMoePlanOut o) {
@@ -234,17 +236,17 @@ __global__ void __launch_bounds__(1024) plan_scan_kernel(uint32_t experts, uint3
     extern __shared__ uint32_t smem[];
     uint32_t *counts = smem, *starts = smem + experts, *sbuf = smem + 2 * experts;
     const uint32_t tid = threadIdx.x;
-    const bool bad = scratch[(size_t)chunks * experts] != 0;
+    const bool bad = scratch[PLAN_FLAG] != 0;
     __syncthreads();
-    if (tid == 0) scratch[(size_t)chunks * experts] = 0;   // the flag is clear again for the next plan
+    if (tid == 0) scratch[PLAN_FLAG] = 0;   // the flag is clear again for the next plan
     for (uint32_t e = tid; e < experts; e += 1024) {        // per expert: counts of earlier chunks
-        uint32_t acc = 0;
+        uint32_t acc = 0, *hist = scratch + PLAN_HIST;
         for (uint32_t c0 = 0; c0 < chunks; c0 += 8) {        // eight loads on their way before the first store: one at a time, 32 chunks took 12 us
             uint32_t v[8];
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++) v[i] = c0 + i < chunks ? scratch[(size_t)(c0 + i) * experts + e] : 0u;
+            for (uint32_t i = 0; i < 8; i++) v[i] = c0 + i < chunks ? hist[(size_t)(c0 + i) * experts + e] : 0u;
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++) { if (c0 + i < chunks) scratch[(size_t)(c0 + i) * experts + e] = acc; acc += v[i]; }
+            for (uint32_t i = 0; i < 8; i++) { if (c0 + i < chunks) hist[(size_t)(c0 + i) * experts + e] = acc; acc += v[i]; }
         }
         counts[e] = acc;
     }
@@ -275,13 +277,13 @@ __global__ void __launch_bounds__(1024) plan_scatter_kernel(uint32_t R, uint32_t
     }
     __syncthreads();
     if (e != 0xffffffffu) {
-        const uint32_t p = starts[e] + scratch[(size_t)blockIdx.x * experts + e] + wcnt[warp * experts + e] + rank_w;
+        const uint32_t p = starts[e] + scratch[PLAN_HIST + (size_t)blockIdx.x * experts + e] + wcnt[warp * experts + e] + rank_w;
         const uint32_t t = i / slots, sl = i - t * slots;
         xmap[p] = t; ymap[p] = t * ystride + sl;
         if (pos) pos[i] = p;
     }
 }
-size_t plan_scratch_words(uint32_t picks, uint32_t experts) { return (size_t)((picks + 1023u) / 1024u) * experts + 1; }
+size_t plan_scratch_words(uint32_t picks, uint32_t experts) { return (size_t)((picks + 1023u) / 1024u) * experts + PLAN_HIST; }
 static bool plan_split(uint32_t picks, uint32_t experts, const uint32_t *scratch, size_t scratch_words, const OmegaGpuMoePlanOut &o) {
     return scratch && picks >= 4096u && o.starts_va && plan_scratch_words(picks, experts) <= scratch_words && (size_t)32 * experts * 2 <= 48 * 1024;
 }
@@ -293,7 +295,7 @@ cudaError_t launch_plan(uint32_t tokens, uint32_t slots, uint32_t experts, uint3
                         const OmegaGpuMoePlanOut &o, cudaStream_t s, uint32_t *scratch, size_t scratch_words) {
     const uint32_t R = tokens * slots, chunks = (R + 1023u) / 1024u;
     if (plan_split(R, experts, scratch, scratch_words, o)) {
-        cudaError_t e = launch_chained(plan_hist_kernel, dim3(chunks), dim3(1024), (size_t)experts * 4, s, R, experts, ids, scratch, chunks);
+        cudaError_t e = launch_chained(plan_hist_kernel, dim3(chunks), dim3(1024), (size_t)experts * 4, s, R, experts, ids, scratch);
         if (e == cudaSuccess) e = launch_chained(plan_scan_kernel, dim3(1), dim3(1024), (size_t)experts * 8 + 96 * 4, s, experts, tile_rows, scratch, chunks, o);
         if (e == cudaSuccess) e = launch_chained(plan_scatter_kernel, dim3(chunks), dim3(1024), (size_t)32 * experts * 2, s, R, slots, experts, ystride, ids, scratch, o, nullptr);
         return e;
