@@ -36,11 +36,11 @@ __global__ void __launch_bounds__(256) combine16_kernel(uint32_t tokens, uint32_
     }
 }
 
-// sorted row p <- codes and scale of row xmap[p]: a warp per row, 16 bytes a lane
-__global__ void __launch_bounds__(256) sort_rows_kernel(uint32_t rows, uint32_t k, const uint32_t *xmap, const int8_t *q, const float *qs, int8_t *__restrict__ q_out, float *__restrict__ qs_out) {
+// sorted row p <- codes and scale of row xmap[p]: a warp per row, 16 bytes a lane. header: the plan's; one that was refused has no rows, and its maps are those of an earlier call
+__global__ void __launch_bounds__(256) sort_rows_kernel(uint32_t rows, uint32_t k, const uint32_t *header, const uint32_t *xmap, const int8_t *q, const float *qs, int8_t *__restrict__ q_out, float *__restrict__ qs_out) {
     griddep_chain();
     const uint32_t lane = threadIdx.x & 31u, p = blockIdx.x * 8u + (threadIdx.x >> 5);
-    if (p >= rows) return;
+    if (p >= min(rows, header[0])) return;
     const uint32_t src = xmap[p];
     const uint4 *from = reinterpret_cast<const uint4 *>(q + (size_t)src * k); uint4 *to = reinterpret_cast<uint4 *>(q_out + (size_t)p * k);
     for (uint32_t w0 = 0; w0 < k / 16u; w0 += 128u) {   // four independent 16-byte loads per lane before the first store
@@ -97,7 +97,7 @@ static int i8_layer_run(OmegaGpuMoeI8Layer *L, uint32_t tokens, const uint16_t *
     // one token's plan is its picks, and the routing writes it (25.8 -> 22.8 us for such a step)
     const bool ok = cuda_ok(launch_score_route(L->route, tokens, logits, 1, 0, L->bias, L->ids, L->wts, s, &o), "route launch") &&
                     (tokens == 1u || cuda_ok(launch_plan(tokens, K, E, K, tr, L->ids, o, s, L->scratch, L->scratch_words), "plan launch")) &&
-                    (!sorted || cuda_ok(launch_chained(sort_rows_kernel, dim3((R + 7u) / 8u), dim3(256), 0, s, R, H, L->xmap, q, qs, L->sq, L->ss), "sort rows launch")) &&
+                    (!sorted || cuda_ok(launch_chained(sort_rows_kernel, dim3((R + 7u) / 8u), dim3(256), 0, s, R, H, L->header, L->xmap, q, qs, L->sq, L->ss), "sort rows launch")) &&
                     cuda_ok(launch_i8_gemm(L->gu, up, s), "gate|up launch") &&
                     cuda_ok(launch_row_q8(R, I, 0, L->gu16, 1, 1, L->aq, L->as, s), "swiglu q8 launch") && cuda_ok(launch_i8_gemm(L->dn, dn, s), "down launch") &&
                     cuda_ok(launch_chained(combine16_kernel, dim3(tokens), dim3(H <= 1024u ? 128 : 256), 0, s, tokens, K, H, L->wts, L->dn16, out32, out16), "combine launch");

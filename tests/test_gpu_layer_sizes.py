@@ -86,3 +86,71 @@ def test_4_bit_layer():
         return out, ids
     same_as_fresh_layers(make, run, api.lib.omega_gpu_moe_w4_layer_free, E, H)
     api.lib.omega_gpu_w4_free(gu); api.lib.omega_gpu_w4_free(dn)
+
+
+class I8Layer(C.Structure):
+    """the 8-bit integer layer's own record, up to the plan's scratch"""
+    _fields_ = ([(n, C.c_void_p) for n in ("gu", "dn")] + [("route", api.MoeRouteConfig)] + [(n, U32) for n in ("hidden", "inter", "max_tokens", "launches")] +
+                [(n, C.c_void_p) for n in ("base", "bias", "wts", "xs", "ss", "as_", "out32", "xq", "sq", "aq", "logits", "x", "gu16", "dn16", "out16", "ids", "counts", "starts", "xmap", "ymap",
+                                           "tiles", "header", "scratch")])
+
+
+class Refusable:
+    """a layer whose next plan can be made to refuse: the word that says an id was out of range is set beforehand"""
+
+    def __init__(self, most):
+        from tests.test_gpu_i8 import codes, config, ok, scales
+        rng = np.random.default_rng(4)
+        self.E, self.H, self.I, self.K = 8, 256, 128, 8
+        rc, self.gu = api.i8_upload(codes(rng, self.E * 2 * self.I, self.H), scales(rng, self.E * 2 * self.I, 0.0005)); ok(rc)
+        rc, self.dn = api.i8_upload(codes(rng, self.E * self.H, self.I), scales(rng, self.E * self.H, 0.0005)); ok(rc)
+        rc, self.h = api.moe_i8_layer_create(self.gu, self.dn, config(self.E, self.K, True), None, most); ok(rc)
+        self.own = C.cast(self.h, C.POINTER(I8Layer)).contents
+        assert (self.own.hidden, self.own.inter, self.own.max_tokens) == (self.H, self.I, most)
+
+    def inputs(self, tokens):
+        rng = np.random.default_rng(tokens)
+        return orc.bf16_bits(rng.normal(0, 1, (tokens, self.E)).astype(np.float32)), orc.bf16_bits(rng.normal(0, 1, (tokens, self.H)).astype(np.float32))
+
+    def copy(self, dst, src, nbytes):
+        import torch
+        torch.cuda.synchronize()
+        assert C.CDLL("libcudart.so.12").cudaMemcpy(C.c_void_p(dst), C.c_void_p(src), C.c_size_t(nbytes), 4) == 0     # 4: either way
+
+    def refuse_next(self):
+        word = np.ones(1, np.uint32)
+        self.copy(self.own.scratch, word.ctypes.data, 4)
+
+    def read(self, at, shape, dtype):
+        out = np.zeros(shape, dtype)
+        self.copy(out.ctypes.data, at, out.nbytes)
+        return out
+
+    def free(self):
+        api.lib.omega_gpu_moe_i8_layer_free(self.h); api.lib.omega_gpu_i8_free(self.gu); api.lib.omega_gpu_i8_free(self.dn)
+
+
+def test_a_refused_plan_moves_no_rows():
+    """the maps are then those of the call before, whose rows may lie past this call's"""
+    import torch
+    from tests.test_gpu_i8 import dev, here, ok
+    m = Refusable(1024)
+    out = torch.zeros((1024, m.H), device="cuda")
+
+    def call(tokens):
+        lg, x = (dev(v) for v in m.inputs(tokens))
+        ok(api.lib.omega_gpu_moe_i8_layer_async(m.h, tokens, lg.data_ptr(), x.data_ptr(), out.data_ptr(), 0, here()))
+        torch.cuda.synchronize()
+        return out[:tokens].clone()
+    call(1024)
+    before = m.read(m.own.sq, (1024 * m.K, m.H), np.int8), m.read(m.own.ss, 1024 * m.K, np.float32)
+    m.refuse_next()
+    call(600)
+    header = m.read(m.own.header, 4, np.uint32)
+    assert list(header) == [0, 0, 0, 2]
+    after = m.read(m.own.sq, (1024 * m.K, m.H), np.int8), m.read(m.own.ss, 1024 * m.K, np.float32)
+    assert all(np.array_equal(a, b) for a, b in zip(before, after))
+    first = call(600)                                                      # the word is clear again
+    assert list(m.read(m.own.header, 4, np.uint32))[3] == 0 and torch.equal(call(600), first)
+    assert not np.array_equal(m.read(m.own.sq, (1024 * m.K, m.H), np.int8), before[0])
+    m.free()
