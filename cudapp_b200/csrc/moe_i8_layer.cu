@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(256) sort_rows_kernel(uint32_t rows, uint32_t 
     if (lane == 0) qs_out[p] = qs[src];
 }
 
+constexpr int I8_REFUSED = 100;   // status of a refused plan: this and the plan's own word, as the FP8 layer reports it
 static size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 }  // namespace b200
@@ -189,14 +190,20 @@ int omega_gpu_moe_i8_layer_bf16(OmegaGpuMoeI8Layer *L, uint32_t tokens, const ui
     if (out_f32) ok = ok && to_host(out_f32, L->out32, xb * 2, s);
     if (ids) ok = ok && to_host(ids, L->ids, rb, s);
     if (wts) ok = ok && to_host(wts, L->wts, rb, s);
-    return ok && omega_gpu_moe_i8_layer_status(L, s) == 0 ? OMEGA_GPU_FP8_OK : OMEGA_GPU_FP8_CHIP_FAIL;
+    if (!ok) return OMEGA_GPU_FP8_CHIP_FAIL;
+    const int status = omega_gpu_moe_i8_layer_status(L, s);
+    if (status > I8_REFUSED) { set_error("i8 layer: routing plan refused (status %d)", status - I8_REFUSED); return OMEGA_GPU_FP8_BAD_ARGS; }
+    return status == 0 ? OMEGA_GPU_FP8_OK : OMEGA_GPU_FP8_CHIP_FAIL;
 }
 
 int omega_gpu_moe_i8_layer_status(OmegaGpuMoeI8Layer *L, void *stream) {
     if (!L) return OMEGA_GPU_FP8_BAD_ARGS;
     Lock l;
-    const int rc = i8_status(L->gu, (cudaStream_t)stream);
-    return rc ? rc : i8_status(L->dn, (cudaStream_t)stream);
+    cudaStream_t s = (cudaStream_t)stream;
+    uint32_t refused = 0;
+    if (!cuda_ok(cudaMemcpyAsync(&refused, L->header + 3, 4, cudaMemcpyDeviceToHost, s), "copy status")) return OMEGA_GPU_FP8_CHIP_FAIL;
+    const int up = i8_status(L->gu, s), down = up ? 0 : i8_status(L->dn, s);   // they wait for s
+    return up ? up : down ? down : refused ? I8_REFUSED + (int)refused : 0;
 }
 
 uint32_t omega_gpu_moe_i8_layer_launches(const OmegaGpuMoeI8Layer *L) { return L ? L->launches : 0; }

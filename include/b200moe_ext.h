@@ -351,7 +351,8 @@ int omega_gpu_moe_i8_layer_q8_async(OmegaGpuMoeI8Layer *l, uint32_t tokens, uint
 /* host buffers; ids / wts optional ([tokens][topk]) */
 int omega_gpu_moe_i8_layer_bf16(OmegaGpuMoeI8Layer *l, uint32_t tokens, const uint16_t *logits_bf16, const uint16_t *x_bf16, uint16_t *out_bf16, float *out_f32,
                                 uint32_t *ids, float *wts);
-/* as omega_gpu_i8_status, of the layer's two tensors */
+/* as omega_gpu_i8_status, of the layer's two tensors; 100 + header[3] when the last call's routing plan was refused (its results are not to be used; the blocking
+ * entry returns BAD_ARGS then) */
 int omega_gpu_moe_i8_layer_status(OmegaGpuMoeI8Layer *l, void *stream);
 uint32_t omega_gpu_moe_i8_layer_launches(const OmegaGpuMoeI8Layer *l);
 

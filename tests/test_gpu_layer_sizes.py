@@ -154,3 +154,23 @@ def test_a_refused_plan_moves_no_rows():
     assert list(m.read(m.own.header, 4, np.uint32))[3] == 0 and torch.equal(call(600), first)
     assert not np.array_equal(m.read(m.own.sq, (1024 * m.K, m.H), np.int8), before[0])
     m.free()
+
+
+def test_a_refused_plan_is_reported():
+    import torch
+    from tests.test_gpu_i8 import dev, here, ok
+    m = Refusable(600)
+    lg, x = m.inputs(600)
+    rc, _, want, _, _ = api.moe_i8_layer_bf16(m.h, lg, x, m.K); ok(rc)
+    want = want.copy()
+    m.refuse_next()
+    rc, _, _, _, _ = api.moe_i8_layer_bf16(m.h, lg, x, m.K)
+    assert rc == api.BAD_ARGS and "refused (status 2)" in api.last_error()
+    m.refuse_next()
+    dl, dx, out = dev(lg), dev(x), torch.zeros((600, m.H), device="cuda")
+    ok(api.lib.omega_gpu_moe_i8_layer_async(m.h, 600, dl.data_ptr(), dx.data_ptr(), out.data_ptr(), 0, here()))
+    assert api.lib.omega_gpu_moe_i8_layer_status(m.h, here()) == 102
+    for tokens in (600, 1):                                                # nothing of it stays
+        rc, _, got, _, _ = api.moe_i8_layer_bf16(m.h, lg[:tokens], x[:tokens], m.K); ok(rc)
+        assert np.array_equal(got.view(np.uint32), want[:tokens].view(np.uint32)) and api.lib.omega_gpu_moe_i8_layer_status(m.h, here()) == 0
+    m.free()
