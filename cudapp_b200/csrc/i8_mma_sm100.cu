@@ -35,7 +35,8 @@ struct I8MmaArgs {
     // box: rows of one load; packed: bf16 rows of a multiple of 8 channels; lag: of a copying warp's stages, how many stay in flight behind the newest, 0 or 1;
     // split: CTAs of a unit; once: weights are read by one tile each and need not stay in L2
     // early: the units and their weights are known before the kernels ahead in the stream have completed
-    uint32_t m, n, k, experts, tiles_most, steps, cblocks, n_cap, stages, tmem_cols, box, packed, lag, early, split, once;
+    // tile_rows: most rows that a tile of a plan may have; x_limit: without a map, rows of x (a tile's rows from there on are left out), else no limit
+    uint32_t m, n, k, experts, tiles_most, tile_rows, x_limit, steps, cblocks, n_cap, stages, tmem_cols, box, packed, lag, early, split, once;
     uint32_t *err;
 };
 
@@ -103,7 +104,10 @@ template <int CG> __device__ __forceinline__ I8Unit i8_unit(const I8MmaArgs &a, 
     const uint32_t t = u / a.cblocks;
     I8Unit r;
     r.c0 = (u - t * a.cblocks) * (128u * CG);
-    if (a.tiles) { const uint4 v = a.tiles[t]; r.expert = min(v.x, a.experts - 1u); r.row0 = v.y; r.cnt = min(v.z, a.n_cap); }   // a plan for other calls must not lead out of this one's buffers
+    if (a.tiles) {   // of a plan that does not fit this call, what the call knows is bounded: experts, rows of a tile, rows of x and their scales. The lengths of maps and of y it does not know
+        const uint4 v = a.tiles[t];
+        r.expert = min(v.x, a.experts - 1u); r.row0 = v.y; r.cnt = min(min(v.z, a.tile_rows), a.x_limit > v.y ? a.x_limit - v.y : 0u);
+    }
     else {   // 16 or 32 rows more or less, so that any number of tiles divides them evenly
         r.expert = 0; r.row0 = (uint32_t)((uint64_t)t * a.steps / a.tiles_most) * (16u * CG);
         r.cnt = min(a.m, (uint32_t)((uint64_t)(t + 1u) * a.steps / a.tiles_most) * (16u * CG)) - r.row0;
@@ -498,7 +502,7 @@ cudaError_t launch_i8_mma(const OmegaGpuI8Tensor *t, const I8Launch &l, cudaStre
     a.once = l.tiles && l.tile_rows <= 64u;
     uint32_t cg = 1;
     if (l.tiles) {
-        a.tiles_most = l.m;
+        a.tiles_most = l.m; a.tile_rows = l.tile_rows; a.x_limit = l.xmap ? 0xffffffffu : l.x_rows;
         cg = !l.xmap && l.tile_rows >= 128u ? 2u : 1u;   // long tiles in pairs: a layer of 4096 tokens 288 us instead of 307, of 1500 tokens 174 instead of 183
         a.n_cap = (l.tile_rows + 16u * cg - 1u) / (16u * cg) * (16u * cg);
     }

@@ -328,7 +328,8 @@ int omega_gpu_i8_gemm(const OmegaGpuI8Tensor *t, uint32_t m, const int8_t *x, co
 /* Grouped by expert: the tensor was uploaded as experts x (n / experts) rows. The rows to multiply are described by a routing plan (omega_gpu_moe_plan_async) made
  * with tile_rows from 1 to 256: tiles u32 x4 {expert, first sorted row, rows <= tile_rows (0: nothing to do), -}, header[2] = number of tiles, at most max_tiles. Row i of a tile is
  * x[xmap[first + i]] with that row's scale (xmap_va 0: x[first + i]); x holds x_rows dense rows. Its result row (n / experts wide) is y[ymap[first + i]]
- * (ymap_va 0: y[first + i]). One launch, nothing allocated. */
+ * (ymap_va 0: y[first + i]). One launch, nothing allocated. first + rows lies inside the maps that are given, and every result row inside y: the call does not know
+ * their lengths. What a plan made for another call is cut to: experts - 1, tile_rows rows in a tile, x_rows rows of x (xmap's values; without it rows from there on are left out). */
 int omega_gpu_i8_gemm_grouped_async(const OmegaGpuI8Tensor *t, uint32_t experts, uint32_t tile_rows, uint32_t max_tiles, uint64_t tiles_va, uint64_t header_va,
                                     uint64_t xmap_va, uint64_t ymap_va, uint64_t x_va, uint32_t x_rows, uint64_t x_scale_va, uint64_t y_bf16_va, uint64_t y_f32_va, void *stream);
 
