@@ -35,8 +35,9 @@ __device__ __forceinline__ uint32_t order_key(float v) {   // larger float, larg
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 __device__ __forceinline__ void push_top2(float v, float &a, float &b) { if (v > a) { b = a; a = v; } else if (v > b) b = v; }
 
-// One warp per token; a lane holds the VPL consecutive experts from lane * VPL, so the lowest lane of equal keys holds the lowest index.
-template <int VPL>
+// One warp per token; a lane holds the VPL consecutive experts from lane * VPL, so the lowest lane of equal keys holds the lowest index. FINE: softmax weights that are not
+// renormalised carry the error of the sum, so its exponentials are better ones (8192 tokens x 256 experts 17.3 us; 16.0 with the fast ones, which the others keep).
+template <int VPL, bool FINE>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32, VPL <= 8 ? 8 : 2) score_route_kernel(const RouteArgs a) {
     griddep_chain();
     extern __shared__ float route_sm[];   // [warp][experts]
@@ -97,6 +98,11 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, VPL <= 8 ? 8 : 2) score_rout
         if (a.sigmoid) return 1.0 / (1.0 + exp(-(double)v));
         return v == -INFINITY ? 0.0 : v == top ? 1.0 : exp((double)v - (double)top);
     };
+    // e^(v - top), off by 3e-7 at most: 2 units of 2^-23 of expf and half a unit of the product with what the subtraction lost
+    auto below_top = [&](float v) {
+        const float d = v - top, t = d - v, lost = (v - (d - t)) - (top + t), e = expf(d);   // d + lost = v - top exactly, where d is finite
+        return e > 0.0f ? fmaf(e, lost, e) : 0.0f;
+    };
 #pragma unroll 1
     for (int exact = 0; exact < 2; exact++) {
         sum = 0.0;
@@ -119,7 +125,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, VPL <= 8 ? 8 : 2) score_rout
             for (int i = 0; i < VPL; i++) s[i] = __fdividef(1.0f, 1.0f + __expf(-l[i]));   // NaN stays NaN
         } else {
 #pragma unroll
-            for (int i = 0; i < VPL; i++) { s[i] = l[i] != l[i] || l[i] == -INFINITY ? 0.0f : l[i] == top ? 1.0f : __expf(l[i] - top); sum += (double)s[i]; }
+            for (int i = 0; i < VPL; i++) { s[i] = l[i] != l[i] || l[i] == -INFINITY ? 0.0f : l[i] == top ? 1.0f : FINE ? below_top(l[i]) : __expf(l[i] - top); sum += (double)s[i]; }
             for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             const float inv = sum > 0.0 ? (float)(1.0 / sum) : 0.0f;
 #pragma unroll
@@ -221,16 +227,18 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, VPL <= 8 ? 8 : 2) score_rout
                 for (uint32_t j = 0; j < n; j++) place += s_cand[warp][j] > mine;
                 my_rank = lane < n ? place : 32u;
                 if (!a.sigmoid) {
-                    // the softmax's sum is of f32 exponentials: less than 4e-7 off. Neighbours that this could make equal, or no longer equal, are left to the second pass
+                    // The softmax's sum may be of f32 exponentials, off by (2 + 1.173 |x|) 2^-23 each and by |x| 2^-24 with the subtraction's rounding: where 1023 experts share one logit, |x| = 5.4
+                    // makes the most of it, 1.1e-6 of the sum. Neighbours that this could make equal, or no longer equal, are left to the second pass; without a bias the sum's error is a
+                    // factor of both and only their roundings count
                     __syncwarp();
                     if (lane < n) s_cand[warp][place] = mine;
                     __syncwarp();
-                    // (rounded to a subnormal number, 4e-7 of a score may be a whole unit of it)
+                    // (rounded to a subnormal number, that much of a score may be a whole unit of it)
                     if (!a.bias && lane < n && place < a.topk && (uint32_t)(mine >> 32) > KEY_NAN) near |= my_s < TINY && my_l != -INFINITY;
                     const uint64_t next = place < a.topk && place + 1u < n ? s_cand[warp][place + 1u] : 0;
                     if ((uint32_t)(next >> 32) > KEY_NAN) {
                         const float v = key_value((uint32_t)(mine >> 32)), w = key_value((uint32_t)(next >> 32));
-                        near |= v != w && !(v - w > 1e-6f * (a.bias ? most : my_s) + (a.bias ? 2.4e-7f * fabsf(v) : 0.0f));
+                        near |= v != w && !(v - w > (a.bias ? 1.5e-6f * most : 1e-6f * my_s) + (a.bias ? 2.4e-7f * fabsf(v) : 0.0f));
                         // equal as they are: the same logit and bias, or near
                         if (v == w) {
                             const uint32_t e = my_id, f = ~(uint32_t)next;
@@ -308,8 +316,12 @@ cudaError_t launch_score_route(const OmegaGpuMoeRouteConfig &c, uint32_t tokens,
     a.bias_vec = bias && ((uintptr_t)bias % 16u) == 0 && c.experts % vpl == 0; a.magic = a.size > 1u ? 0xffffffffu / a.size + 1u : 0u;
     const size_t smem = (size_t)ROUTE_WARPS * c.experts * 4;
     const dim3 grid((tokens + ROUTE_WARPS - 1) / ROUTE_WARPS), block(ROUTE_WARPS * 32);
-    return vpl == 4u ? launch_chained(score_route_kernel<4>, grid, block, smem, s, a) : vpl == 8u ? launch_chained(score_route_kernel<8>, grid, block, smem, s, a)
-         : vpl == 16u ? launch_chained(score_route_kernel<16>, grid, block, smem, s, a) : launch_chained(score_route_kernel<32>, grid, block, smem, s, a);
+#define ROUTE(VPL) return !a.sigmoid && !a.norm ? launch_chained(score_route_kernel<VPL, true>, grid, block, smem, s, a) : launch_chained(score_route_kernel<VPL, false>, grid, block, smem, s, a)
+    if (vpl == 4u) ROUTE(4);
+    if (vpl == 8u) ROUTE(8);
+    if (vpl == 16u) ROUTE(16);
+    ROUTE(32);
+#undef ROUTE
 }
 
 }  // namespace b200

@@ -40,3 +40,48 @@ def test_grouped_product_of_a_plan_that_does_not_fit(tile_rows, gathered, n):
     assert np.all(np.abs(y.cpu().numpy() - want) <= 3 * EPS24 * np.abs(want))
     assert np.all(np.abs(y16.double().cpu().numpy() - want) <= (2.0 ** -8 * (1 + 2 ** -7) + 4 * EPS24) * np.abs(want))
     api.lib.omega_gpu_i8_free(t)
+
+
+@pytest.mark.parametrize("E", [128, 1024])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_softmax_weights_of_many_equal_logits(E, bf16):
+    """one expert ahead and the rest at one logit: the errors of the exponentials are the same and add up. The weights that are not renormalised carry the sum's error, 4e-7 at
+    most, and one rounding of their own"""
+    import torch
+    g = torch.Generator(device="cuda"); g.manual_seed(E)
+    T = 40000
+    top = torch.rand(T, generator=g, device="cuda") * 4 - 2
+    l = (top - 3 - 5 * torch.rand(T, generator=g, device="cuda"))[:, None].repeat(1, E)
+    l[torch.arange(T, device="cuda"), torch.randint(E, (T,), generator=g, device="cuda")] = top
+    if bf16:
+        l = l.bfloat16()
+    for K in (1, 3):
+        ids, w = torch.zeros((T, K), dtype=torch.int32, device="cuda"), torch.zeros((T, K), device="cuda")
+        ok(api.lib.omega_gpu_moe_route_async(api.MoeRouteConfig(E, K, api.SCORE_SOFTMAX, 1, 0, 1, 0, 1.0), T, l.data_ptr(), int(bf16), 0, 0, ids.data_ptr(), w.data_ptr(), here()))
+        want = torch.softmax(l.double(), 1).gather(1, ids.long())
+        assert torch.equal(ids[:, 0].long(), l.argmax(1))
+        assert float(((w.double() - want).abs() / want).max()) <= 4e-7 + EPS24
+
+
+def test_softmax_of_logits_whose_difference_is_no_number():
+    """the largest and the lowest value of the type, infinities: no NaN from the difference's own rounding"""
+    big = np.finfo(np.float32).max
+    l = np.full((4, 64), -3.0, np.float32)
+    l[0] = -big; l[0, 7] = big; l[1, 9] = np.inf; l[2, ::2] = -np.inf; l[2, 3] = big; l[3] = -big; l[3, 5] = 2e38
+    for norm in (0, 1):
+        rc, ids, w = api.moe_route(api.MoeRouteConfig(64, 3, api.SCORE_SOFTMAX, 1, 0, 1, norm, 1.0), l); ok(rc)
+        want, wants = ref.route(l, 3, False, norm=bool(norm))
+        assert np.array_equal(ids, want) and np.array_equal(w, wants)
+
+
+@pytest.mark.parametrize("E", [128, 1024])
+def test_softmax_picks_next_to_a_tie_of_score_and_bias(E):
+    """one expert ahead, the rest at one logit, and a bias that lifts another expert to where the two change places as the logit ahead goes through neighbouring floats"""
+    for base, low in ((0.95, -4.92), (0.0, -5.9), (-1.5, -6.5)):
+        l = np.full((240, E), low, np.float32)
+        l[:, 9] = (np.float32(base).view(np.uint32) + np.arange(240, dtype=np.uint32) * 2).view(np.float32) if base else np.linspace(-1e-5, 1e-5, 240).astype(np.float32)
+        p = np.exp(l[120].astype(np.float64)); p /= p.sum()
+        bias = np.zeros(E, np.float32); bias[4] = p[9] - p[4]
+        rc, ids, w = api.moe_route(api.MoeRouteConfig(E, 2, api.SCORE_SOFTMAX, 1, 0, 1, 1, 1.0), l, bias); ok(rc)
+        want, _ = ref.route(l, 2, False, bias)
+        assert np.array_equal(ids, want) and len(set(ids[:, 0].tolist())) == 2
