@@ -21,8 +21,8 @@
 
 namespace b200 {
 
-constexpr uint32_t I8_EPI = 16, I8_STAGES = 12, I8_N_MAX = 256;   // epilogue warps, most stages, most rows of a tile
-constexpr uint32_t i8_threads(bool gather) { return 128 + 32 * I8_EPI + (gather ? 128 : 0); }
+constexpr uint32_t I8_EPI = 16, I8_STAGES = 12, I8_N_MAX = 256, I8_TEAM = 4;   // epilogue warps, most stages, most rows of a tile, warps that copy rows
+constexpr uint32_t i8_threads(bool gather) { return 128 + 32 * I8_EPI + (gather ? 32 * I8_TEAM : 0); }
 constexpr uint32_t I8_OUT_ROW = 80, I8_OUT = 16 * I8_OUT_ROW;     // an epilogue warp's 16 result rows of 32 bf16 channels; 80 bytes apart: neither side meets a bank twice
 constexpr size_t I8_SMEM = 214 * 1024;                            // dynamic shared memory of every form: stages, result rows, alignment
 constexpr uint32_t I8_ROOM = (uint32_t)I8_SMEM - 1024u - I8_EPI * I8_OUT;   // the stages' part
@@ -341,12 +341,12 @@ __global__ void __launch_bounds__(i8_threads(GATHER), 1) i8_mma_kernel(const __g
             if (CG == 1) hand_back();
         }
     } else if (GATHER && warp >= 4 + I8_EPI) {
-        // ---------------------------------------------------------------- row copies: each of `team` warps fills every team-th stage
+        // ---------------------------------------------------------------- row copies: each of the team's warps fills every team-th stage
         // No more warps than stages: a warp that waits for a place in the ring has then had one since the place's last turn began, and the barrier's parity tells the turns apart.
-        constexpr uint32_t team = 4;
+        constexpr uint32_t team = I8_TEAM;
         static_assert(I8_ROOM / (A_TILE + I8_N_MAX * 128) >= team, "a ring of as many stages as copying warps");
-        // A stage is passed on once its copies have landed and are fenced for the tensor cores' reads; a.lag = 1: when the warp's next stage has been requested,
-        // which takes more than 2 * team stages in the ring (every wait for a free stage is then for one that has been passed on).
+        // A stage is passed on once its copies have landed and are fenced for the tensor cores' reads; a.lag = 1: when the warp's next stage has been requested. In a ring of
+        // 2 * team stages or more the place of stage i + team is free once stage i - team or an earlier one has been multiplied, which was passed on when stage i was requested.
         if constexpr (GATHER) {
             const uint32_t me = warp - (4 + I8_EPI), c = lane & 7u, r0 = lane >> 3;
             uint32_t *src = s_src[me];
@@ -517,7 +517,7 @@ cudaError_t launch_i8_mma(const OmegaGpuI8Tensor *t, const I8Launch &l, cudaStre
     a.packed = l.y16 && !l.y32 && l.n % 8u == 0;
     const bool two = i8_two_blocks(cg, per_cta, (t->k + 127u) / 128u, a.split, l.xmap != nullptr);
     a.stages = I8_ROOM / ((A_TILE + per_cta * 128u) * (two ? 2u : 1u)); if (a.stages > I8_STAGES) a.stages = I8_STAGES;
-    a.lag = a.stages > 7u;
+    a.lag = a.stages >= 2u * I8_TEAM;
     a.tmem_cols = 32; while (a.tmem_cols < 2u * a.n_cap) a.tmem_cols *= 2;
     CUtensorMap w, x;
     if (!make_tmap_u8(&w, t->w, t->n, t->k, 128) || !make_tmap_u8(&x, l.x, l.x_rows, t->k, a.box, l.x_stride)) return cudaErrorInvalidValue;
