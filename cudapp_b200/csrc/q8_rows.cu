@@ -192,7 +192,9 @@ cudaError_t launch_norm_q8(uint32_t tokens, uint32_t hidden, float eps, const vo
 }
 template <bool GATE, typename X>
 static cudaError_t row_launch(uint32_t rows, uint32_t n, size_t stride, const X *x, int8_t *q, float *s, cudaStream_t st_) {
-    const uint32_t most = 4u * (uint32_t)(st().sm_count ? st().sm_count : 148);   // as many as are resident at once
+    // Four CTAs an SM: by its registers the gate of bf16 rows up to 768 columns has as many resident, forms with fewer values a thread up to eight, those with more one to three;
+    // of these the CTAs that do not fit start as others end, and only then request their first row
+    const uint32_t most = 4u * (uint32_t)(st().sm_count ? st().sm_count : 148);
 #define ROW(WV, VV) { const uint32_t ctas = (WV) == 1 ? (rows + 7) / 8 : rows; return launch_chained(row_q8_kernel<WV, VV, GATE, X>, dim3(ctas < most ? ctas : most), dim3(256), 0, st_, rows, n, stride, x, q, s); }
     if (n <= 256) ROW(1, 1);
     if (n <= 512) ROW(1, 2);
