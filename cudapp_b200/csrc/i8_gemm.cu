@@ -196,6 +196,7 @@ int omega_gpu_i8_gemm_grouped_async(const OmegaGpuI8Tensor *t, uint32_t experts,
                                     uint64_t xmap_va, uint64_t ymap_va, uint64_t x_va, uint32_t x_rows, uint64_t x_scale_va, uint64_t y_bf16_va, uint64_t y_f32_va, void *stream) {
     if (!t || !experts || t->n % experts || !tile_rows || tile_rows > 256 || !max_tiles || !tiles_va || !header_va || !x_va || !x_rows || !x_scale_va || (!y_bf16_va && !y_f32_va)) return OMEGA_GPU_FP8_BAD_ARGS;
     if (max_tiles > I8_MAX_ROWS || x_rows > I8_MAX_ROWS) return OMEGA_GPU_FP8_TOO_LARGE;
+    if ((uint64_t)max_tiles * ((t->n / experts + 127u) / 128u) > 0x7fffffffull) { set_error("i8 grouped: %u tiles of %u channels are more than 2^31 - 1 blocks of 128", max_tiles, t->n / experts); return OMEGA_GPU_FP8_TOO_LARGE; }
     if (((tiles_va | x_va | y_bf16_va | y_f32_va) & 15u) || ((header_va | xmap_va | ymap_va | x_scale_va) & 3u)) return OMEGA_GPU_FP8_BAD_ARGS;
     const int ready = async_ready();
     if (ready != OMEGA_GPU_FP8_OK) return ready;

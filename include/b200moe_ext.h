@@ -326,7 +326,8 @@ int omega_gpu_i8_gemm_async(const OmegaGpuI8Tensor *t, uint32_t m, uint64_t x_va
 /* host buffers, dense */
 int omega_gpu_i8_gemm(const OmegaGpuI8Tensor *t, uint32_t m, const int8_t *x, const float *x_scale, uint16_t *y_bf16, float *y_f32);
 /* Grouped by expert: the tensor was uploaded as experts x (n / experts) rows. The rows to multiply are described by a routing plan (omega_gpu_moe_plan_async) made
- * with tile_rows from 1 to 256: tiles u32 x4 {expert, first sorted row, rows <= tile_rows (0: nothing to do), -}, header[2] = number of tiles, at most max_tiles. Row i of a tile is
+ * with tile_rows from 1 to 256: tiles u32 x4 {expert, first sorted row, rows <= tile_rows (0: nothing to do), -}, header[2] = number of tiles, at most max_tiles (max_tiles times
+ * the 128-channel blocks of an expert below 2^31, else TOO_LARGE). Row i of a tile is
  * x[xmap[first + i]] with that row's scale (xmap_va 0: x[first + i]); x holds x_rows dense rows. Its result row (n / experts wide) is y[ymap[first + i]]
  * (ymap_va 0: y[first + i]). One launch, nothing allocated. first + rows lies inside the maps that are given, and every result row inside y: the call does not know
  * their lengths. What a plan made for another call is cut to: experts - 1, tile_rows rows in a tile, x_rows rows of x (xmap's values; without it rows from there on are left out). */

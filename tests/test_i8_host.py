@@ -95,3 +95,9 @@ def test_no_device_fails_loudly():
     assert L.omega_gpu_moe_route_async(cfg(), 1, V, 0, 0, 0, V, V, 0) == api.CHIP_FAIL
     assert L.omega_gpu_swiglu_q8_async(1, 64, V, 1, V, V, 0) == api.CHIP_FAIL
     assert api.moe_route(cfg(), np.zeros((2, 64), np.float32))[0] == api.CHIP_FAIL
+
+
+def test_too_many_blocks_of_a_plan():
+    t, call = C.pointer(Tensor(4 * 1024, 32)), L.omega_gpu_i8_gemm_grouped_async
+    assert call(t, 4, 16, 1 << 30, V, V, 0, 0, V, 3, V, V, 0, 0) == api.TOO_LARGE and "blocks of 128" in api.last_error()
+    assert call(t, 4, 16, 1 << 28, V, V, 0, 0, V, 3, V, V, 0, 0) == api.TOO_LARGE
