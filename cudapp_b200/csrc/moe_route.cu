@@ -61,7 +61,12 @@ __device__ __forceinline__ bool plan_tables(uint32_t experts, uint32_t tile_rows
                                             const OmegaGpuMoePlanOut &o, bool bad) {
     const uint32_t tid = threadIdx.x;
     uint32_t *hdr = reinterpret_cast<uint32_t *>(o.header_va);
-    if (bad) {   // refuse: nothing but the status word is written
+    const Seg32 zero = {0, 0, 0, 0, 0};
+    if (bad) {   // refuse: no rows, no segments (a product that walks the records would take the plan before for this one), nothing else is written
+        for (uint32_t z = tid; z < experts; z += 1024) {
+            if (o.seg_a_va) reinterpret_cast<Seg32 *>(o.seg_a_va)[z] = zero;
+            if (o.seg_b_va) reinterpret_cast<Seg32 *>(o.seg_b_va)[z] = zero;
+        }
         if (tid == 0) { hdr[0] = 0; hdr[1] = 0; hdr[2] = 0; hdr[3] = 2; }
         return false;
     }
@@ -94,7 +99,6 @@ __device__ __forceinline__ bool plan_tables(uint32_t experts, uint32_t tile_rows
     }
     // records past the last non-empty expert: zero count, skipped by the consumers
     for (uint32_t z = segs_total + tid; z < experts; z += 1024) {
-        const Seg32 zero = {0, 0, 0, 0, 0};
         if (o.seg_a_va) reinterpret_cast<Seg32 *>(o.seg_a_va)[z] = zero;
         if (o.seg_b_va) reinterpret_cast<Seg32 *>(o.seg_b_va)[z] = zero;
     }

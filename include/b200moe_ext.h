@@ -40,7 +40,8 @@ int omega_gpu_moe_topk_async(uint32_t tokens, uint32_t experts, uint32_t topk, i
  * xmap[rows+8] = token, ymap[rows+8] = token*ystride+slot (8 zero pads), seg: 32-byte records for the non-empty
  * experts in ascending id built from the two directories ({w_va, s_va} per expert), records past the last
  * non-empty expert up to `experts` zeroed; tiles: one {expert, row0, cnt} u32 x4 entry per `tile_rows` slice of
- * a segment (tile_rows 0 = none); header u32[8] = {rows, segments, tiles, status, w, 0, 0, 0}; status 2 = id out of range; word w is
+ * a segment (tile_rows 0 = none); header u32[8] = {rows, segments, tiles, status, w, 0, 0, 0}; status 2 = id out of range (no
+ * rows: the first three words are 0 and the segment records zeroed, counts, maps and tiles are left as they were); word w is
  * left as it is (the kernels that consume a plan record an expired bounded wait there: zero it once, when the buffer is made). */
 typedef struct {
     uint64_t counts_va, starts_va, xmap_va, ymap_va;

@@ -174,3 +174,54 @@ def test_a_refused_plan_is_reported():
         rc, _, got, _, _ = api.moe_i8_layer_bf16(m.h, lg[:tokens], x[:tokens], m.K); ok(rc)
         assert np.array_equal(got.view(np.uint32), want[:tokens].view(np.uint32)) and api.lib.omega_gpu_moe_i8_layer_status(m.h, here()) == 0
     m.free()
+
+
+@pytest.mark.parametrize("E,T", [(5, 9), (700, 40)])
+def test_a_refused_plan_has_no_segments(E, T):
+    """records of the plan before would be taken for its own by a product that walks them"""
+    import torch
+    rng = np.random.default_rng(E)
+    S, R = 3, T * 3
+    ids = rng.integers(0, E, (T, S)).astype(np.int32)
+    z = lambda n, t=torch.int32: torch.zeros(n, dtype=t, device="cuda")     # noqa: E731
+    counts, starts, xmap, ymap, seg_a, seg_b, header = z(E), z(E), z(R + 8), z(R + 8), z(8 * E), z(8 * E), z(8)
+    table = torch.arange(16, 16 + 2 * E, device="cuda")
+    o = api.MoePlanOut(counts.data_ptr(), starts.data_ptr(), xmap.data_ptr(), ymap.data_ptr(), seg_a.data_ptr(), table.data_ptr(), seg_b.data_ptr(), table.data_ptr(), 0, header.data_ptr())
+
+    def plan(v):
+        d = torch.from_numpy(v).cuda()
+        rc = api.lib.omega_gpu_moe_plan_async(U32(T), U32(S), U32(E), U32(S), U32(0), C.c_uint64(d.data_ptr()), C.byref(o), C.c_void_p(torch.cuda.current_stream().cuda_stream))
+        assert rc == 0, api.last_error()
+        torch.cuda.synchronize()
+    assert api.lib.omega_gpu_moe_topk_bf16(U32(1), U32(1), U32(1), C.c_int(1), api._p(np.zeros(1, np.uint16)), api._p(np.zeros(1, np.uint32)), api._p(np.zeros(1, np.float32))) == 0   # opens the device
+    plan(ids)
+    assert header[3] == 0 and int((seg_a.view(E, 8)[:, 5] > 0).sum()) == len(np.unique(ids)) and torch.equal(seg_a, seg_b)
+    kept = [t.clone() for t in (counts, starts, xmap, ymap)]
+    bad = ids.copy(); bad[T // 2, 1] = E
+    plan(bad)
+    assert header[:4].tolist() == [0, 0, 0, 2] and not seg_a.any() and not seg_b.any()
+    assert all(torch.equal(a, b) for a, b in zip(kept, (counts, starts, xmap, ymap)))
+
+
+def test_fp8_layer_on_the_exact_engine_after_a_refused_plan():
+    """a call of 2 tokens with an id outside the layer, after one of 64: nothing is read through the 64 tokens' maps, and the next call is right"""
+    import torch
+    from tests.test_gpu_layer import build_layer, free_layer
+    E, H, I, K = 8, 512, 256, 2
+    m = build_layer(np.random.default_rng(6), E, H, I, 64, api.ENGINE_FMA, K)
+    g = torch.Generator(device="cuda"); g.manual_seed(1)
+    x, w, out = torch.randn((64, H), generator=g, device="cuda").bfloat16(), torch.rand((64, K), generator=g, device="cuda"), torch.zeros((64, H), device="cuda")
+    ids = torch.stack([torch.randperm(E, generator=torch.Generator().manual_seed(i))[:K] for i in range(64)]).int().cuda()
+    s, V = C.c_void_p(torch.cuda.current_stream().cuda_stream), lambda t: C.c_uint64(t.data_ptr())
+
+    def call(n, ids):
+        xs = x[:n].clone()
+        rc = api.lib.omega_gpu_moe_layer_routed_async(m["layer"], U32(n), V(ids), V(w), V(xs), V(out), C.c_uint64(0), s); assert rc == 0, api.last_error()
+        return api.lib.omega_gpu_moe_layer_status(m["layer"], s)
+    assert call(64, ids) == 0
+    want = out.clone()
+    bad = ids[:2].clone(); bad[1, 0] = E
+    assert call(2, bad) == 102
+    assert call(2, ids) == 0 and torch.equal(out[:2], want[:2])
+    assert call(64, ids) == 0 and torch.equal(out, want)
+    free_layer(m)
