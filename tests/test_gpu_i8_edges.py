@@ -85,3 +85,89 @@ def test_softmax_picks_next_to_a_tie_of_score_and_bias(E):
         rc, ids, w = api.moe_route(api.MoeRouteConfig(E, 2, api.SCORE_SOFTMAX, 1, 0, 1, 1, 1.0), l, bias); ok(rc)
         want, _ = ref.route(l, 2, False, bias)
         assert np.array_equal(ids, want) and len(set(ids[:, 0].tolist())) == 2
+
+
+# ------------------------------------------------------------------ the layer
+@pytest.mark.parametrize("T,E,H,I,K", [(1, 1, 16, 16, 1), (3, 1, 16, 16, 1), (70, 2, 16, 48, 2), (1, 1024, 64, 32, 32), (40, 1024, 64, 32, 32), (300, 1024, 64, 32, 16), (1, 40, 16, 8192, 32), (2, 2, 16384, 16, 1)])
+def test_layer_of_extreme_shapes(T, E, H, I, K):
+    from tests.test_gpu_i8 import Layer, bits, check_rows, quantised
+    L = Layer(T + E, E, H, I, K, T)
+    rng = np.random.default_rng(T)
+    lg, x = bits(rng.normal(0, 1, (T, E)).astype(np.float32)), bits(rng.normal(0, 1, (T, H)).astype(np.float32))
+    rc, o16, o32, ids, w = api.moe_i8_layer_bf16(L.h, lg, x, K); ok(rc)
+    q, s = quantised(x)
+    check_rows(q, s, api.bf16_to_f32(x).astype(np.float64), 0.0)
+    wids, ww, want = L.want(lg, q, s)
+    assert np.array_equal(ids, wids) and np.all(np.abs(w - ww) <= (K + 5) * EPS24 * ww)
+    # A code may fall one step off with a chance of 127 * 2 * 2e-6 + 1.3e-4 (see LAYER_REL); as many of the I T K codes as that makes likely, and four deviations and one more. The codes' rms is
+    # 30 or more in short rows; in one of thousands the largest of the products is further out, 8
+    n = I * T * K; mean = n * (127 * 2 * 2e-6 + 1.3e-4)
+    off = np.ceil(mean + 4 * np.sqrt(mean) + 1)
+    assert np.linalg.norm(o32 - want) <= np.sqrt(off / n) / (30 if I <= 256 else 8) * np.linalg.norm(want)
+    L.free()
+
+
+def test_layer_rows_that_are_not_finite_stay_by_themselves():
+    from tests.test_gpu_i8 import Layer, bits
+    for T, E, K in ((40, 8, 2), (700, 8, 8)):
+        L = Layer(3, E, 256, 128, K, T)
+        rng = np.random.default_rng(T)
+        lg, x = bits(rng.normal(0, 1, (T, E)).astype(np.float32)), bits(rng.normal(0, 1, (T, 256)).astype(np.float32))
+        rc, _, want, _, _ = api.moe_i8_layer_bf16(L.h, lg, x, K); ok(rc)
+        want = want.copy()
+        bad = x.copy(); bad[5, 17] = 0x7fc0; bad[11, 3] = 0x7f80; bad[T - 1, 0] = 0xff80
+        rc, o16, o32, _, _ = api.moe_i8_layer_bf16(L.h, lg, bad, K); ok(rc)
+        rest = np.ones(T, bool); rest[[5, 11, T - 1]] = False
+        assert np.isnan(o32[~rest]).all() and np.isnan(api.bf16_to_f32(o16[~rest])).all()
+        assert np.array_equal(o32[rest].view(np.uint32), want[rest].view(np.uint32))
+        L.free()
+
+
+def test_captured_layer_between_eager_calls_of_other_sizes():
+    """a step of 700 tokens and one of one token, captured; between their replays the same layer runs 1024, 600 and 3 tokens"""
+    import torch
+    from tests.test_gpu_i8 import Layer
+    E, H, I, K, most = 8, 256, 128, 8, 1024
+    L = Layer(7, E, H, I, K, most)
+    g = torch.Generator(device="cuda"); g.manual_seed(2)
+    lg, x = torch.randn((most, E), generator=g, device="cuda").bfloat16(), torch.randn((most, H), generator=g, device="cuda").bfloat16()
+    out = {n: torch.zeros((n, H), device="cuda") for n in (700, 1, 1024, 600, 3)}
+
+    def call(n):
+        ok(api.lib.omega_gpu_moe_i8_layer_async(L.h, n, lg.data_ptr(), x.data_ptr(), out[n].data_ptr(), 0, here()))
+    want = {}
+    for n in out:
+        call(n); torch.cuda.synchronize(); want[n] = out[n].clone()
+    graphs = {}
+    for n in (700, 1):
+        graphs[n] = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graphs[n]):
+            call(n)
+    for n in (700, 1024, 700, 1, 600, 700, 700, 3, 1, 1024, 600, 700):
+        out[n].fill_(-7)
+        graphs[n].replay() if n in graphs else call(n)
+        torch.cuda.synchronize()
+        assert torch.equal(out[n], want[n]) and api.lib.omega_gpu_moe_i8_layer_status(L.h, here()) == 0
+    L.free()
+
+
+def test_two_layers_on_the_same_tensors_at_once():
+    import torch
+    from tests.test_gpu_i8 import Layer, config
+    E, H, I, K = 16, 512, 256, 4
+    L = Layer(9, E, H, I, K, 400)
+    rc, other = api.moe_i8_layer_create(L.tgu, L.tdn, config(E, K, True), L.bias, 30); ok(rc)
+    g = torch.Generator(device="cuda"); g.manual_seed(4)
+    jobs = []
+    for h, T in ((L.h, 400), (other, 30)):
+        lg, x = torch.randn((T, E), generator=g, device="cuda").bfloat16(), torch.randn((T, H), generator=g, device="cuda").bfloat16()
+        jobs.append((h, T, lg, x, [torch.zeros((T, H), device="cuda") for _ in range(30)], torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for i in range(30):
+        for h, T, lg, x, outs, s in jobs:
+            ok(api.lib.omega_gpu_moe_i8_layer_async(h, T, lg.data_ptr(), x.data_ptr(), outs[i].data_ptr(), 0, s.cuda_stream))
+    torch.cuda.synchronize()
+    for h, T, lg, x, outs, s in jobs:
+        assert outs[0].any() and all(torch.equal(outs[0], o) for o in outs[1:]) and api.lib.omega_gpu_moe_i8_layer_status(h, here()) == 0
+    api.lib.omega_gpu_moe_i8_layer_free(other)
+    L.free()
